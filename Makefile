@@ -4,6 +4,9 @@
 HIPCC    ?= /opt/rocm/bin/hipcc
 ARCH     ?= gfx950
 CXXFLAGS ?= -O3 -std=c++17 -fPIC -Wall -Wno-unused-function -Wno-unused-variable
+# no packed fp32 instructions: -O3 forms them by itself from ordinary float code, and some of their
+# forms have given wrong results on this hardware (the host pass warns that it does not know the feature)
+NOPACK   := -Xclang -target-feature -Xclang -packed-fp32-ops
 SRC      := $(wildcard autovc_amd/csrc/*.hip)
 HDR      := $(wildcard autovc_amd/csrc/*.h) include/autovc_hip.h include/autovc_hip_debug.h
 OBJ      := $(patsubst autovc_amd/csrc/%.hip,build/%.o,$(SRC))
@@ -18,7 +21,7 @@ SCHED_lstm := -mllvm -amdgpu-sched-strategy=max-ilp
 
 build/%.o: autovc_amd/csrc/%.hip $(HDR) Makefile
 	@mkdir -p build
-	$(HIPCC) --offload-arch=$(ARCH) $(CXXFLAGS) $(SCHED_$*) -c $< -o $@
+	$(HIPCC) --offload-arch=$(ARCH) $(CXXFLAGS) $(NOPACK) $(SCHED_$*) -c $< -o $@
 
 $(LIB): $(OBJ)
 	$(HIPCC) --offload-arch=$(ARCH) -shared -fPIC $(OBJ) -o $@
@@ -42,7 +45,7 @@ SAN_BIN   := tests/host_sanitize/abi_driver
 
 build/sanitize/%.o: autovc_amd/csrc/%.hip $(HDR)
 	@mkdir -p build/sanitize
-	$(HIPCC) --offload-arch=$(ARCH) $(SAN_FLAGS) -c $< -o $@
+	$(HIPCC) --offload-arch=$(ARCH) $(SAN_FLAGS) $(NOPACK) -c $< -o $@
 
 $(SAN_BIN): $(SAN_OBJ) tests/host_sanitize/abi_driver.cpp include/autovc_hip.h include/autovc_hip_debug.h
 	$(HIPCC) --offload-arch=$(ARCH) $(SAN_FLAGS) $(SAN_OBJ) tests/host_sanitize/abi_driver.cpp -o $@
@@ -55,5 +58,5 @@ sanitize: $(SAN_BIN)
 # diagnostic build with in-kernel s_memtime stamps (never shipped): diag/libautovc_hip_stamps.so
 stamps:
 	@mkdir -p diag
-	$(HIPCC) --offload-arch=$(ARCH) $(CXXFLAGS) -DAVC_STAMPS -shared $(SRC) -o diag/libautovc_hip_stamps.so
+	$(HIPCC) --offload-arch=$(ARCH) $(CXXFLAGS) $(NOPACK) -DAVC_STAMPS -shared $(SRC) -o diag/libautovc_hip_stamps.so
 .PHONY: stamps

@@ -8,6 +8,7 @@ if [ "$1" = build ]; then
     d=abd_${v##*:}; mkdir -p $d
     defs=""; for f in $(echo ${v%%:*} | tr '+' ' '); do defs="$defs -DAVC_GEMM_$f=1"; done
     /opt/rocm/bin/hipcc --offload-arch=gfx950 -O3 -std=c++17 -fPIC -Wno-unused-function -Wno-unused-variable \
+      -Xclang -target-feature -Xclang -packed-fp32-ops \
       $defs -c autovc_amd/csrc/gemm.hip -o $d/gemm.o
     /opt/rocm/bin/hipcc --offload-arch=gfx950 -shared -fPIC $(ls build/*.o | grep -v '/gemm.o$') $d/gemm.o \
       -o $d/libautovc_hip.so
