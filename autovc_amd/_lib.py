@@ -21,6 +21,8 @@ _P = ctypes.c_void_p
 _I = ctypes.c_int
 _F = ctypes.c_float
 _Z = ctypes.c_size_t
+_L = ctypes.c_long
+_LL = ctypes.c_longlong
 
 # name -> argtypes (restype is int unless listed in _RESTYPES)
 _SIGS = {
@@ -132,8 +134,19 @@ _SIGS = {
     "avc_wavernn_generate": [_P, _P, _I, _P, _P, _I, _I, _I, _I, ctypes.c_ulonglong, _P, _P, _P, _P, _P],
     "avc_wavernn_fold_shape": [ctypes.c_long, _I, _I, _I, ctypes.POINTER(ctypes.c_long),
                                ctypes.POINTER(ctypes.c_long)],
+    "avc_gated_recurrence_states": [_I, _I, _I, _I],
+    "avc_gated_recurrence_workspace": [_I, _I, _I, _I, _I],
+    "avc_gated_recurrence_forward": [_I, _I, _I, _I, _I, _P, _L, _P, _P, _P, _L, _P, _P, _P, _Z, _P],
+    "avc_gated_recurrence_backward": [_I, _I, _I, _I, _I, _P, _L, _P, _P, _P, _L, _P, _P, _L, _P, _P, _Z, _P],
+    "avc_gated_recurrence_step": [_I, _I, _I, _P, _L, _P, _P, _P, _L, _P],
+    "avc_token_log_probs_workspace": [_I, _L, _L, _I],
+    "avc_token_log_probs_forward": [_I, _L, _L, _P, _L, _P, _LL, _I, _P, _P, _P, _P, _P, _P, _Z, _P],
+    "avc_token_log_probs_backward": [_I, _L, _L, _P, _L, _P, _LL, _P, _P, _P, _P, _L, _P],
+    "avc_dropout": [_I, _L, _L, _P, _L, _P, _L, ctypes.c_double, _P, ctypes.c_uint, _P, _L, _P],
 }
-_RESTYPES = {"avc_last_error": ctypes.c_char_p, "avc_act_frag_bytes": _Z, "avc_conv_wgrad_image_bytes": _Z}
+_RESTYPES = {"avc_last_error": ctypes.c_char_p, "avc_act_frag_bytes": _Z, "avc_conv_wgrad_image_bytes": _Z,
+             "avc_gated_recurrence_states": _Z, "avc_gated_recurrence_workspace": _Z,
+             "avc_token_log_probs_workspace": _Z}
 
 _lib = None
 _lock = threading.RLock()
@@ -220,6 +233,10 @@ def ptr(t) -> int | None:
     if not t.is_contiguous():
         raise ValueError("autovc_amd kernels need contiguous tensors")
     return t.data_ptr()
+
+
+# element types of the sequence-model operators (AVC_DTYPE_*)
+DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 
 
 TIMING_CLASSES = {"gemm": 0, "lstm_step_fwd": 1, "lstm_step_bwd": 2, "lstm32": 3, "dft64": 4, "lstm2_persist": 5,

@@ -265,6 +265,13 @@ __device__ __forceinline__ void amax_update(unsigned* w, float v) {
   if (__hip_atomic_load(w, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) < u) atomicMax(w, u);
 }
 
+// 64-bit finaliser of the counter-based streams (the vocoder's sampling, dropout)
+__device__ __forceinline__ unsigned long long mix64(unsigned long long z) {
+  z = (z ^ (z >> 30)) * 0xBF58476D1CE4E5B9ull;
+  z = (z ^ (z >> 27)) * 0x94D049BB133111EBull;
+  return z ^ (z >> 31);
+}
+
 __device__ __forceinline__ float sigmoidf_(float x) { return 1.0f / (1.0f + expf(-x)); }
 
 // One BatchNorm statistics partial (S = column sum of its n rows, Q = sum of squares about its own

@@ -1,0 +1,593 @@
+// Gated linear recurrence over time-major frames: f = sigmoid(g_f), z = tanh(g_c), o = sigmoid(g_o),
+//   h_t = f_t h_{t-1} + (1 - f_t) z_t,   y_t = o_t h_t.
+// Its time loop is linear in h, so a stretch of frames acts on the state before it as
+// h -> A h + B with A = prod f and B the stretch's own state from zero, and stretches compose:
+// time is split over waves (and, where there are few rows, over workgroups) and joined.
+//
+// The backward runs the same way from the end.  With e_t the gradient of h_t and c_t = f_t e_t what
+// frame t hands to frame t - 1:  e_t = o_t dy_t + c_{t+1},  c_t = f_t e_t  (c behind the last frame
+// is the gradient of the final state), a stretch acts as c -> A c + B' with the same A, and
+//   dg_f = e_t (h_{t-1} - z) f (1 - f),  dg_c = e_t (1 - f)(1 - z^2),  dg_o = dy h_t o (1 - o).
+// h is formed again from states that the forward keeps every kStateStep frames.
+//
+// Everything but the loaded and stored elements is fp32.  1 - f is never formed by subtraction.
+#include "typed.h"
+
+namespace avc {
+namespace {
+
+constexpr int kStateStep = 64;  // frames between the states that the forward keeps for the backward
+constexpr int kS = 8;           // frames of a wave's stretch, all in registers
+constexpr int kW = 8;           // waves of a workgroup = stretches of its chunk
+constexpr int kChunk = kS * kW;
+static_assert(kStateStep % kS == 0, "a kept state is the state before some wave's stretch");
+
+struct RecArgs {
+  int T, B, H, dirs;
+  const void* gates;
+  long ldg;
+  const int* lengths;
+  const float* h0;   // [D][B][H]
+  void* y;
+  long ldy;
+  float* hT;         // [D][B][H]
+  float* states;     // [ceil(T / kStateStep)][D][B][H]
+  const void* dy;
+  long lddy;
+  const float* dhT;
+  void* dgates;
+  long lddg;
+  float* dh0;
+  float* agg;        // [nseg][2][D][B][H]: A and B (B') of each segment
+  int nseg, seg_chunks;
+  int log_g, nct;    // lanes of a wave per row (log2), channel tiles per row
+};
+
+// Forget gate and its complement.  Below -80 (f < 2e-35) the exponential is held there, so that
+// neither it nor the reciprocal leaves the normal range; a NaN passes.
+__device__ __forceinline__ void forget_gate(float g, float& f, float& i) {
+  const float gc = g < -80.0f ? -80.0f : g;
+  const float e = __expf(-gc);
+  f = __builtin_amdgcn_rcpf(1.0f + e);
+  i = e * f;
+}
+// tanh for 16-bit inputs: a shorter polynomial than gate_tanh's, error below 1e-6 relative
+__device__ __forceinline__ float tanh_short(float x) {
+  const float ax = fabsf(x), x2 = x * x;
+  float p = fmaf(x2, -0.0539682540f, 0.133333333f);
+  p = fmaf(p, x2, -0.333333333f);
+  const float small = fmaf(x * x2, p, x);
+  const float big = 1.0f - 2.0f * __builtin_amdgcn_rcpf(1.0f + __expf(2.0f * ax));
+  return ax < 0.15f ? small : copysignf(big, x);
+}
+template <typename E>
+__device__ __forceinline__ float candidate(float x) {
+  return sizeof(E) == 4 ? gate_tanh(x) : tanh_short(x);
+}
+
+// Where a lane works: VEC channels of one row b in one direction.  Rows narrower than a wave share
+// it.  The last vector of a row is moved back to end at H (channels that two lanes share get the
+// same value twice), so no vector is cut; lanes past the row or the batch repeat its last place
+// and store nothing.
+template <typename E, int VEC>
+struct Place {
+  int b, j, d, len;
+  bool ok, rev;
+  __device__ explicit Place(const RecArgs& a) {
+    const int lane = threadIdx.x & 63, g = 1 << a.log_g;
+    const int cv = (blockIdx.x % a.nct) * g + (lane & (g - 1));
+    const int row = (int)(blockIdx.x / a.nct) * (64 >> a.log_g) + (lane >> a.log_g);
+    ok = cv * VEC < a.H && row < a.B;
+    j = min(cv * VEC, a.H - VEC);
+    b = min(row, a.B - 1);
+    d = blockIdx.z;
+    rev = a.dirs == 2 || d == 1;
+    len = a.lengths ? min(max(a.lengths[b], 0), a.T) : a.T;
+  }
+  __device__ long state(const RecArgs& a) const { return ((long)d * a.B + b) * a.H + j; }
+};
+
+// frame of step s (0 .. T-1 in the direction's own order), and whether it is inside the sequence;
+// the frame is one that exists, also where it is not live
+template <bool RAGGED>
+__device__ __forceinline__ int frame_of(const RecArgs& a, int s, bool rev, int len, bool& live) {
+  const int sc = min(s, a.T - 1);
+  const int t = rev ? a.T - 1 - sc : sc;
+  live = s < a.T && (!RAGGED || t < len);
+  return RAGGED ? min(t, max(len - 1, 0)) : t;
+}
+
+template <typename E, int VEC, bool RAGGED>
+__global__ __launch_bounds__(kW * 64) void recurrence_forward_kernel(RecArgs a) {
+  const Place<E, VEC> at(a);
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  __shared__ float part[2][kW][2][64][VEC];
+  const E* g = static_cast<const E*>(a.gates) + (long)at.b * a.ldg + (long)at.d * 3 * a.H + at.j;
+  E* y = static_cast<E*>(a.y) + (long)at.b * a.ldy + (long)at.d * a.H + at.j;
+  const long gstep = (long)a.B * a.ldg, ystep = (long)a.B * a.ldy;
+  const long st = at.state(a), nstate = (long)(a.dirs == 3 ? 2 : 1) * a.B * a.H;
+
+  float h[VEC];
+#pragma unroll
+  for (int v = 0; v < VEC; ++v) h[v] = a.h0 ? a.h0[st + v] : 0.0f;
+  for (int q = 0; q < (int)blockIdx.y; ++q) {  // the segments before this one, in order
+    const float* p = a.agg + (long)q * 2 * nstate + st;
+#pragma unroll
+    for (int v = 0; v < VEC; ++v) h[v] = fmaf(p[v], h[v], p[nstate + v]);
+  }
+
+  const int first = blockIdx.y * a.seg_chunks;
+  const int last = min(first + a.seg_chunks, (a.T + kChunk - 1) / kChunk);
+  Vec<E, VEC> rf[kS], rc[kS], ro[kS];
+  auto load = [&](int chunk) {
+    const int s0 = chunk * kChunk + wave * kS;
+    if (chunk >= last || s0 >= a.T) return;
+#pragma unroll
+    for (int k = 0; k < kS; ++k) {
+      bool live;
+      const E* p = g + frame_of<RAGGED>(a, s0 + k, at.rev, at.len, live) * gstep;
+      rf[k] = vload<E, VEC>(p);
+      rc[k] = vload<E, VEC>(p + a.H);
+      ro[k] = vload<E, VEC>(p + 2 * a.H);
+    }
+  };
+  load(first);
+  for (int chunk = first; chunk < last; ++chunk) {
+    const int s0 = chunk * kChunk + wave * kS;
+    float prod[kS][VEC], loc[kS][VEC], o[kS][VEC];
+    float A[VEC], Bv[VEC];
+#pragma unroll
+    for (int v = 0; v < VEC; ++v) A[v] = 1.0f, Bv[v] = 0.0f;
+    if (s0 < a.T) {
+#pragma unroll
+      for (int k = 0; k < kS; ++k) {
+        bool live;
+        frame_of<RAGGED>(a, s0 + k, at.rev, at.len, live);
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) {
+          float f, i;
+          forget_gate((float)rf[k].v[v], f, i);
+          const float z = candidate<E>((float)rc[k].v[v]);
+          o[k][v] = gate_sigmoid((float)ro[k].v[v]);
+          Bv[v] = live ? fmaf(f, Bv[v], i * z) : Bv[v];
+          A[v] = live ? A[v] * f : A[v];
+          prod[k][v] = A[v];
+          loc[k][v] = Bv[v];
+        }
+      }
+    }
+    float (*mine)[2][64][VEC] = part[chunk & 1];
+#pragma unroll
+    for (int v = 0; v < VEC; ++v) mine[wave][0][lane][v] = A[v], mine[wave][1][lane][v] = Bv[v];
+    load(chunk + 1);
+    __syncthreads();
+    float hin[VEC];
+#pragma unroll
+    for (int w = 0; w < kW; ++w) {
+#pragma unroll
+      for (int v = 0; v < VEC; ++v) {
+        if (w == wave) hin[v] = h[v];
+        h[v] = fmaf(mine[w][0][lane][v], h[v], mine[w][1][lane][v]);
+      }
+    }
+    if (s0 < a.T && at.ok) {
+      if (a.states && s0 % kStateStep == 0) {
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) a.states[(long)(s0 / kStateStep) * nstate + st + v] = hin[v];
+      }
+#pragma unroll
+      for (int k = 0; k < kS; ++k) {
+        if (s0 + k >= a.T) break;
+        const int t = at.rev ? a.T - 1 - s0 - k : s0 + k;
+        const bool live = !RAGGED || t < at.len;
+        float out[VEC];
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) out[v] = live ? o[k][v] * fmaf(prod[k][v], hin[v], loc[k][v]) : 0.0f;
+        vstore<E, VEC>(y + t * ystep, out);
+      }
+    }
+  }
+  if (a.hT && last == (a.T + kChunk - 1) / kChunk && wave == 0 && at.ok) {
+#pragma unroll
+    for (int v = 0; v < VEC; ++v) a.hT[st + v] = h[v];
+  }
+}
+
+template <typename E, int VEC, bool RAGGED>
+__global__ __launch_bounds__(kW * 64) void recurrence_backward_kernel(RecArgs a) {
+  const Place<E, VEC> at(a);
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  __shared__ float part[2][kW][3][64][VEC];
+  const E* g = static_cast<const E*>(a.gates) + (long)at.b * a.ldg + (long)at.d * 3 * a.H + at.j;
+  const E* dy = static_cast<const E*>(a.dy) + (long)at.b * a.lddy + (long)at.d * a.H + at.j;
+  E* dg = static_cast<E*>(a.dgates) + (long)at.b * a.lddg + (long)at.d * 3 * a.H + at.j;
+  const long gstep = (long)a.B * a.ldg, dystep = (long)a.B * a.lddy, dgstep = (long)a.B * a.lddg;
+  const long st = at.state(a), nstate = (long)(a.dirs == 3 ? 2 : 1) * a.B * a.H;
+
+  float c[VEC];  // what the frames behind this chunk hand back
+#pragma unroll
+  for (int v = 0; v < VEC; ++v) c[v] = a.dhT ? a.dhT[st + v] : 0.0f;
+  for (int q = a.nseg - 1; q > (int)blockIdx.y; --q) {
+    const float* p = a.agg + (long)q * 2 * nstate + st;
+#pragma unroll
+    for (int v = 0; v < VEC; ++v) c[v] = fmaf(p[v], c[v], p[nstate + v]);
+  }
+
+  const int first = blockIdx.y * a.seg_chunks;
+  const int last = min(first + a.seg_chunks, (a.T + kChunk - 1) / kChunk);
+  Vec<E, VEC> rf[kS], rc[kS], ro[kS], ry[kS];
+  float hs[VEC];
+  auto load = [&](int chunk) {
+    const int s0 = chunk * kChunk + wave * kS;
+    if (chunk < first) return;
+#pragma unroll
+    for (int v = 0; v < VEC; ++v) hs[v] = a.states[(long)(chunk * (kChunk / kStateStep)) * nstate + st + v];
+    if (s0 >= a.T) return;
+#pragma unroll
+    for (int k = 0; k < kS; ++k) {
+      bool live;
+      const int t = frame_of<RAGGED>(a, s0 + k, at.rev, at.len, live);
+      const E* p = g + t * gstep;
+      rf[k] = vload<E, VEC>(p);
+      rc[k] = vload<E, VEC>(p + a.H);
+      ro[k] = vload<E, VEC>(p + 2 * a.H);
+      ry[k] = vload<E, VEC>(dy + t * dystep);
+    }
+  };
+  load(last - 1);
+  for (int chunk = last - 1; chunk >= first; --chunk) {
+    const int s0 = chunk * kChunk + wave * kS;
+    float f[kS][VEC], i[kS][VEC], z[kS][VEC], o[kS][VEC], d[kS][VEC];
+    float A[VEC], Bv[VEC], Cv[VEC];
+#pragma unroll
+    for (int v = 0; v < VEC; ++v) A[v] = 1.0f, Bv[v] = 0.0f, Cv[v] = 0.0f;
+    if (s0 < a.T) {
+#pragma unroll
+      for (int k = 0; k < kS; ++k) {
+        bool live;
+        frame_of<RAGGED>(a, s0 + k, at.rev, at.len, live);
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) {
+          // a frame behind the end keeps the state and hands every gradient through
+          forget_gate((float)rf[k].v[v], f[k][v], i[k][v]);
+          z[k][v] = candidate<E>((float)rc[k].v[v]);
+          o[k][v] = gate_sigmoid((float)ro[k].v[v]);
+          d[k][v] = (float)ry[k].v[v];
+          if (RAGGED || k > 0) {
+            f[k][v] = live ? f[k][v] : 1.0f;
+            i[k][v] = live ? i[k][v] : 0.0f;
+            z[k][v] = live ? z[k][v] : 0.0f;
+            o[k][v] = live ? o[k][v] : 0.0f;
+            d[k][v] = live ? d[k][v] : 0.0f;
+          }
+          Bv[v] = fmaf(f[k][v], Bv[v], i[k][v] * z[k][v]);
+          A[v] *= f[k][v];
+        }
+      }
+#pragma unroll
+      for (int k = kS - 1; k >= 0; --k)
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) Cv[v] = f[k][v] * fmaf(o[k][v], d[k][v], Cv[v]);
+    }
+    float (*mine)[3][64][VEC] = part[chunk & 1];
+    float hin[VEC], cin[VEC];
+#pragma unroll
+    for (int v = 0; v < VEC; ++v) {
+      mine[wave][0][lane][v] = A[v], mine[wave][1][lane][v] = Bv[v], mine[wave][2][lane][v] = Cv[v];
+      hin[v] = hs[v];
+    }
+    load(chunk - 1);
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < kW; ++w)
+#pragma unroll
+      for (int v = 0; v < VEC; ++v)
+        if (w < wave) hin[v] = fmaf(mine[w][0][lane][v], hin[v], mine[w][1][lane][v]);
+#pragma unroll
+    for (int w = kW - 1; w >= 0; --w)
+#pragma unroll
+      for (int v = 0; v < VEC; ++v) {
+        if (w == wave) cin[v] = c[v];
+        c[v] = fmaf(mine[w][0][lane][v], c[v], mine[w][2][lane][v]);
+      }
+    if (s0 < a.T && at.ok) {
+      float h[kS + 1][VEC];
+#pragma unroll
+      for (int v = 0; v < VEC; ++v) h[0][v] = hin[v];
+#pragma unroll
+      for (int k = 0; k < kS; ++k)
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) h[k + 1][v] = fmaf(f[k][v], h[k][v], i[k][v] * z[k][v]);
+#pragma unroll
+      for (int k = kS - 1; k >= 0; --k) {
+        float df[VEC], dc[VEC], dov[VEC];
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) {
+          const float e = fmaf(o[k][v], d[k][v], cin[v]);
+          cin[v] = f[k][v] * e;
+          df[v] = cin[v] * i[k][v] * (h[k][v] - z[k][v]);
+          dc[v] = e * i[k][v] * fmaf(-z[k][v], z[k][v], 1.0f);
+          dov[v] = d[k][v] * h[k + 1][v] * fmaf(-o[k][v], o[k][v], o[k][v]);
+        }
+        if (s0 + k < a.T) {
+          const int t = at.rev ? a.T - 1 - s0 - k : s0 + k;
+          E* p = dg + t * dgstep;
+          vstore<E, VEC>(p, df);
+          vstore<E, VEC>(p + a.H, dc);
+          vstore<E, VEC>(p + 2 * a.H, dov);
+        }
+      }
+    }
+  }
+  if (a.dh0 && first == 0 && wave == 0 && at.ok) {
+#pragma unroll
+    for (int v = 0; v < VEC; ++v) a.dh0[st + v] = c[v];
+  }
+}
+
+// What one segment of time does to the state before it (BACK: to the gradient behind it): each
+// wave walks a run of chunks' stretches of its own, then the waves' runs are joined in order.
+template <typename E, int VEC, bool RAGGED, bool BACK>
+__global__ __launch_bounds__(kW * 64) void recurrence_segment_kernel(RecArgs a) {
+  const Place<E, VEC> at(a);
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  __shared__ float part[kW][2][64][VEC];
+  const E* g = static_cast<const E*>(a.gates) + (long)at.b * a.ldg + (long)at.d * 3 * a.H + at.j;
+  const E* dy = BACK ? static_cast<const E*>(a.dy) + (long)at.b * a.lddy + (long)at.d * a.H + at.j : nullptr;
+  const long gstep = (long)a.B * a.ldg, dystep = (long)a.B * a.lddy;
+  const long st = at.state(a), nstate = (long)(a.dirs == 3 ? 2 : 1) * a.B * a.H;
+  // seg_chunks chunks of kW stretches: seg_chunks stretches in a row for each wave
+  const int n = a.seg_chunks;
+  const int base = ((int)blockIdx.y * n * kW + wave * n) * kS;
+  float A[VEC], Bv[VEC];
+#pragma unroll
+  for (int v = 0; v < VEC; ++v) A[v] = 1.0f, Bv[v] = 0.0f;
+  Vec<E, VEC> r0[kS], r1[kS], r2[kS];
+  auto load = [&](int q) {
+    const int s0 = base + (BACK ? n - 1 - q : q) * kS;
+    if (q >= n || s0 >= a.T) return;
+#pragma unroll
+    for (int k = 0; k < kS; ++k) {
+      bool live;
+      const int t = frame_of<RAGGED>(a, s0 + k, at.rev, at.len, live);
+      const E* p = g + t * gstep;
+      r0[k] = vload<E, VEC>(p);
+      if (BACK) {
+        r1[k] = vload<E, VEC>(p + 2 * a.H);
+        r2[k] = vload<E, VEC>(dy + t * dystep);
+      } else {
+        r1[k] = vload<E, VEC>(p + a.H);
+      }
+    }
+  };
+  load(0);
+  for (int q = 0; q < n; ++q) {
+    const int s0 = base + (BACK ? n - 1 - q : q) * kS;
+    float f[kS][VEC], u[kS][VEC];
+    if (s0 < a.T) {
+#pragma unroll
+      for (int k = 0; k < kS; ++k) {
+        bool live;
+        frame_of<RAGGED>(a, s0 + k, at.rev, at.len, live);
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) {
+          float i;
+          forget_gate((float)r0[k].v[v], f[k][v], i);
+          u[k][v] = BACK ? gate_sigmoid((float)r1[k].v[v]) * (float)r2[k].v[v]
+                         : i * candidate<E>((float)r1[k].v[v]);
+          f[k][v] = live ? f[k][v] : 1.0f;
+          u[k][v] = live ? u[k][v] : 0.0f;
+        }
+      }
+    }
+    load(q + 1);
+    if (s0 < a.T) {
+#pragma unroll
+      for (int kk = 0; kk < kS; ++kk) {
+        const int k = BACK ? kS - 1 - kk : kk;
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) {
+          Bv[v] = BACK ? f[k][v] * (u[k][v] + Bv[v]) : fmaf(f[k][v], Bv[v], u[k][v]);
+          A[v] *= f[k][v];
+        }
+      }
+    }
+  }
+#pragma unroll
+  for (int v = 0; v < VEC; ++v) part[wave][0][lane][v] = A[v], part[wave][1][lane][v] = Bv[v];
+  __syncthreads();
+  if (wave == 0 && at.ok) {
+    float* p = a.agg + (long)blockIdx.y * 2 * nstate + st;
+#pragma unroll
+    for (int v = 0; v < VEC; ++v) {
+      float A2 = 1.0f, B2 = 0.0f;
+#pragma unroll
+      for (int ww = 0; ww < kW; ++ww) {
+        const int w = BACK ? kW - 1 - ww : ww;
+        B2 = fmaf(part[w][0][lane][v], B2, part[w][1][lane][v]);
+        A2 *= part[w][0][lane][v];
+      }
+      p[v] = A2;
+      p[nstate + v] = B2;
+    }
+  }
+}
+
+// One frame of every row: the served form.
+template <typename E, int VEC>
+__global__ __launch_bounds__(256) void recurrence_step_kernel(int B, int H, const E* gates, long ldg, const float* h,
+                                                              float* h_out, E* y, long ldy) {
+  const int nv = (H + VEC - 1) / VEC;
+  const long id = (long)blockIdx.x * 256 + threadIdx.x;
+  const int b = (int)(id / nv);
+  if (b >= B) return;
+  // (no shared vectors here: with h_out = h a channel computed twice could be read after its
+  // first write)
+  const int j = (int)(id % nv) * VEC;
+  const E* g = gates + (long)b * ldg + j;
+  const int n = min(VEC, H - j);
+  const long st = (long)b * H + j;
+  float out[VEC], hn[VEC];
+  Vec<E, VEC> rf, rc, ro;
+  float hv[VEC];
+  if (n == VEC) {
+    rf = vload<E, VEC>(g), rc = vload<E, VEC>(g + H), ro = vload<E, VEC>(g + 2 * H);
+    const Vec<float, VEC> t = vload<float, VEC>(h + st);
+#pragma unroll
+    for (int v = 0; v < VEC; ++v) hv[v] = t.v[v];
+  } else {
+#pragma unroll
+    for (int v = 0; v < VEC; ++v) {
+      const int w = min(v, n - 1);
+      rf.v[v] = g[w], rc.v[v] = g[H + w], ro.v[v] = g[2 * H + w], hv[v] = h[st + w];
+    }
+  }
+#pragma unroll
+  for (int v = 0; v < VEC; ++v) {
+    float f, i;
+    forget_gate((float)rf.v[v], f, i);
+    hn[v] = fmaf(f, hv[v], i * candidate<E>((float)rc.v[v]));
+    out[v] = gate_sigmoid((float)ro.v[v]) * hn[v];
+  }
+  E* yo = y + (long)b * ldy + j;
+  if (n == VEC) {
+    vstore<float, VEC>(h_out + st, hn);
+    vstore<E, VEC>(yo, out);
+  } else {
+#pragma unroll
+    for (int v = 0; v < VEC; ++v)
+      if (v < n) h_out[st + v] = hn[v], yo[v] = static_cast<E>(out[v]);
+  }
+}
+
+template <typename E>
+constexpr int wide() { return sizeof(E) == 4 ? 2 : 4; }
+
+// Segments of time: with enough row tiles to fill the chip each workgroup walks its rows' whole
+// time; with fewer, time is cut into as many pieces as bring the grid there.
+int segments(int T, int B, int H, int D, int vec, int* seg_chunks) {
+  const int chunks = (T + kChunk - 1) / kChunk;
+  int log_g = 0;
+  while (log_g < 6 && (vec << log_g) < H) ++log_g;
+  const long tiles = (long)D * ((H + (vec << log_g) - 1) / (vec << log_g)) * ((B + (64 >> log_g) - 1) / (64 >> log_g));
+  long n = tiles >= 256 ? 1 : 512 / tiles;
+  if (n > chunks) n = chunks;
+  *seg_chunks = (int)((chunks + n - 1) / n);
+  return (chunks + *seg_chunks - 1) / *seg_chunks;
+}
+
+template <typename E, int VEC, bool BACK>
+int run_recurrence(RecArgs a, size_t ws_bytes, hipStream_t s) {
+  const int D = a.dirs == 3 ? 2 : 1;
+  a.log_g = 0;
+  while (a.log_g < 6 && (VEC << a.log_g) < a.H) ++a.log_g;
+  a.nct = (a.H + (VEC << a.log_g) - 1) / (VEC << a.log_g);
+  const int rows = 64 >> a.log_g;
+  a.nseg = segments(a.T, a.B, a.H, D, VEC, &a.seg_chunks);
+  const size_t need = a.nseg > 1 ? (size_t)a.nseg * 2 * D * a.B * a.H * sizeof(float) : 0;
+  AVC_CHECK_ARG(ws_bytes >= need && (need == 0 || a.agg), "workspace smaller than avc_gated_recurrence_workspace");
+  const long tiles = (long)a.nct * ((a.B + rows - 1) / rows);
+  AVC_CHECK_ARG(tiles < (1L << 32) / (kW * 64), "B * H too large");
+  const dim3 grid((unsigned)tiles, a.nseg, D);
+  if (a.nseg > 1) {
+    if (a.lengths) recurrence_segment_kernel<E, VEC, true, BACK><<<grid, kW * 64, 0, s>>>(a);
+    else recurrence_segment_kernel<E, VEC, false, BACK><<<grid, kW * 64, 0, s>>>(a);
+    AVC_LAUNCH_CHECK();
+  }
+  if constexpr (BACK) {
+    if (a.lengths) recurrence_backward_kernel<E, VEC, true><<<grid, kW * 64, 0, s>>>(a);
+    else recurrence_backward_kernel<E, VEC, false><<<grid, kW * 64, 0, s>>>(a);
+  } else {
+    if (a.lengths) recurrence_forward_kernel<E, VEC, true><<<grid, kW * 64, 0, s>>>(a);
+    else recurrence_forward_kernel<E, VEC, false><<<grid, kW * 64, 0, s>>>(a);
+  }
+  AVC_LAUNCH_CHECK();
+  return AVC_OK;
+}
+
+int check_shape(int dtype, int T, int B, int H, int dirs, long ldg) {
+  AVC_CHECK_ARG(dtype_ok(dtype), "dtype is one of AVC_DTYPE_F32, _BF16, _F16");
+  AVC_CHECK_ARG(T >= 1 && B >= 0 && H >= 1, "T >= 1, B >= 0, H >= 1");
+  AVC_CHECK_ARG(T <= 1 << 30 && B <= 1 << 30 && H <= 1 << 28, "T, B or H too large");
+  AVC_CHECK_ARG(dirs >= 1 && dirs <= 3, "dirs is 1 (forward), 2 (reverse) or 3 (both)");
+  AVC_CHECK_ARG(ldg >= (long)(dirs == 3 ? 6 : 3) * H, "a gate row is narrower than its gates");
+  return AVC_OK;
+}
+
+}  // namespace
+}  // namespace avc
+
+using namespace avc;
+
+extern "C" size_t avc_gated_recurrence_states(int T, int B, int H, int dirs) {
+  if (T < 0 || B < 0 || H < 1 || dirs < 1 || dirs > 3) return 0;
+  return (size_t)(T / kStateStep + (T % kStateStep != 0)) * (dirs == 3 ? 2 : 1) * B * H;
+}
+
+extern "C" size_t avc_gated_recurrence_workspace(int dtype, int T, int B, int H, int dirs) {
+  if (!dtype_ok(dtype) || T < 1 || B < 1 || H < 1 || dirs < 1 || dirs > 3) return 0;
+  const int D = dirs == 3 ? 2 : 1;
+  const int wide_vec = dtype == AVC_DTYPE_F32 ? wide<float>() : wide<__bf16>();
+  int sc;
+  const int n = segments(T, B, H, D, H >= wide_vec ? wide_vec : 1, &sc);
+  return n > 1 ? (size_t)n * 2 * D * B * H * sizeof(float) : 0;
+}
+
+extern "C" int avc_gated_recurrence_forward(int dtype, int T, int B, int H, int dirs, const void* gates, long ldg,
+                                            const float* h0, const int* lengths, void* y, long ldy, float* hT,
+                                            float* states, void* workspace, size_t workspace_bytes, void* stream) {
+  AVC_TRY(check_shape(dtype, T, B, H, dirs, ldg));
+  const int D = dirs == 3 ? 2 : 1;
+  AVC_CHECK_ARG(ldy >= (long)D * H, "an output row is narrower than D * H");
+  if (B == 0) return AVC_OK;
+  hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+  AVC_CHECK_ARG(gates && y, "gates and y are needed");
+  RecArgs a{};
+  a.T = T, a.B = B, a.H = H, a.dirs = dirs, a.gates = gates, a.ldg = ldg, a.lengths = lengths, a.h0 = h0;
+  a.y = y, a.ldy = ldy, a.hT = hT, a.states = states, a.agg = static_cast<float*>(workspace);
+  return with_dtype(dtype, [&](auto e) {
+    using E = decltype(e);
+    return H >= wide<E>() ? run_recurrence<E, wide<E>(), false>(a, workspace_bytes, s)
+                          : run_recurrence<E, 1, false>(a, workspace_bytes, s);
+  });
+}
+
+extern "C" int avc_gated_recurrence_backward(int dtype, int T, int B, int H, int dirs, const void* gates, long ldg,
+                                             const int* lengths, const float* states, const void* dy, long lddy,
+                                             const float* dhT, void* dgates, long lddg, float* dh0, void* workspace,
+                                             size_t workspace_bytes, void* stream) {
+  AVC_TRY(check_shape(dtype, T, B, H, dirs, ldg));
+  const int D = dirs == 3 ? 2 : 1;
+  AVC_CHECK_ARG(lddy >= (long)D * H && lddg >= (long)D * 3 * H, "a gradient row is narrower than its contents");
+  if (B == 0) return AVC_OK;
+  hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+  AVC_CHECK_ARG(gates && dy && dgates && states, "gates, states, dy and dgates are needed");
+  RecArgs a{};
+  a.T = T, a.B = B, a.H = H, a.dirs = dirs, a.gates = gates, a.ldg = ldg, a.lengths = lengths;
+  a.states = const_cast<float*>(states), a.dy = dy, a.lddy = lddy, a.dhT = dhT, a.dgates = dgates, a.lddg = lddg;
+  a.dh0 = dh0, a.agg = static_cast<float*>(workspace);
+  return with_dtype(dtype, [&](auto e) {
+    using E = decltype(e);
+    return H >= wide<E>() ? run_recurrence<E, wide<E>(), true>(a, workspace_bytes, s)
+                          : run_recurrence<E, 1, true>(a, workspace_bytes, s);
+  });
+}
+
+extern "C" int avc_gated_recurrence_step(int dtype, int B, int H, const void* gates, long ldg, const float* h,
+                                         float* h_out, void* y, long ldy, void* stream) {
+  AVC_TRY(check_shape(dtype, 1, B, H, 1, ldg));
+  AVC_CHECK_ARG(ldy >= H, "an output row is narrower than H");
+  if (B == 0) return AVC_OK;
+  AVC_CHECK_ARG(gates && h && h_out && y, "gates, h, h_out and y are needed");
+  hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+  return with_dtype(dtype, [&](auto e) {
+    using E = decltype(e);
+    constexpr int VEC = 4;
+    const long n = (long)B * ((H + VEC - 1) / VEC);
+    AVC_CHECK_ARG(n < (1L << 32) - 256, "B * H too large");
+    recurrence_step_kernel<E, VEC><<<(unsigned)((n + 255) / 256), 256, 0, s>>>(
+        B, H, static_cast<const E*>(gates), ldg, h, h_out, static_cast<E*>(y), ldy);
+    AVC_LAUNCH_CHECK();
+    return AVC_OK;
+  });
+}

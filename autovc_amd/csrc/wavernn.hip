@@ -486,11 +486,6 @@ __global__ __launch_bounds__(256) void wr_fc_kernel(WrStep a) {
 }
 
 // counter-based uniform in [1e-5, 1 - 1e-5] (oracle/wavernn_oracle.py:uniforms, the same bits)
-__device__ __forceinline__ unsigned long long mix64(unsigned long long z) {
-  z = (z ^ (z >> 30)) * 0xBF58476D1CE4E5B9ull;
-  z = (z ^ (z >> 27)) * 0x94D049BB133111EBull;
-  return z ^ (z >> 31);
-}
 __device__ __forceinline__ float uniform_draw(unsigned long long seed, int r, int i, int d) {
   const unsigned long long base = mix64((seed + 1ull) * 0x9E3779B97F4A7C15ull);
   const unsigned long long ctr = ((unsigned long long)r << 40) | ((unsigned long long)(unsigned)i << 8) | (unsigned)d;

@@ -14,6 +14,7 @@ import torch
 
 from . import _lib
 from ._lib import ACT_NONE, ACT_RELU, ACT_TANH, call, ptr
+from .sequence import dropout, gated_recurrence, gated_recurrence_step, token_log_probs
 
 F32 = 4  # bytes
 
@@ -572,4 +573,5 @@ def gemm(a, b, bias=None, a_trans=False, b_trans=False):
 
 __all__ = ["FramesFromMel", "MelFromFrames", "ConvBNAct", "LSTMLayer", "BiLSTMLayer", "Codes",
            "DecoderInput", "Linear", "Loss", "mse_loss", "l1_loss", "overlap_average", "gemm",
+           "gated_recurrence", "gated_recurrence_step", "token_log_probs", "dropout",
            "ACT_NONE", "ACT_RELU", "ACT_TANH"]

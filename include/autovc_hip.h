@@ -8,7 +8,8 @@
  * point names the reference module/lines whose arithmetic it replaces.
  *
  * Conventions
- *   - All tensors are fp32, borrowed device pointers (the caller owns every buffer).
+ *   - All tensors are fp32 (the sequence-model operators also take bf16 and fp16), borrowed device
+ *     pointers (the caller owns every buffer).
  *   - Activations are TIME-MAJOR "frame rows": element (t, b, c) of a [T*B][C] row-major matrix
  *     at ((t*B + b)*C + c).  Mels/codes crossing the Python boundary keep the reference's
  *     channel-first (B, 80, T) / (B, n_codes) layouts; the glue kernels convert.
@@ -398,6 +399,73 @@ int avc_wavernn_generate(avc_context* ctx, const int* dims, int T, const float* 
  * per-step path (autovc_hip_debug.h: avc_wavernn_persist). */
 int avc_wavernn_fallbacks(void);
 int avc_wavernn_persist_eligible(int rows, int rnn_dims, int fc_dims);
+
+/* ---- sequence-model operators ----------------------------------------------------------------
+ * These take fp32, bf16 or fp16 elements (AVC_DTYPE_*), each value rounded once where it is
+ * stored; states, statistics and sums are fp32.  They keep nothing in a context and take scratch
+ * memory from the caller (sizes from the _workspace calls; it may be shared by calls of one stream,
+ * not by calls that can run at the same time).  Row strides (ld*) are in elements; rows may begin
+ * at any element.  No two buffers of a call may overlap unless its comment says so. */
+#define AVC_DTYPE_F32 0
+#define AVC_DTYPE_BF16 1
+#define AVC_DTYPE_F16 2
+
+/* Gated linear recurrence, the LSTM layer's (nn.LSTM at decoder.py:37,53, encoder.py:51) linear
+ * relative, computed by a scan over time:
+ *   f = sigmoid(g_f)  z = tanh(g_c)  o = sigmoid(g_o)
+ *   h_t = f_t h_{t-1} + (1 - f_t) z_t      y_t = o_t h_t
+ *   dirs     1 = t = 0 .. T-1, 2 = t = T-1 .. 0, 3 = both (D = 2; direction 0 runs forward)
+ *   gates    [T*B] rows of stride ldg, a row holding [D][3][H]: pre-activations f, c, o
+ *   h0, hT   [D][B][H] fp32, state before the first and after the last frame of each direction's own
+ *            order (h0 NULL = 0, hT may be NULL)
+ *   lengths  [B] (NULL = all T; values are held to 0 .. T): frames t >= lengths[b] are not used, their
+ *            y and dgates are 0, and the state passes them unchanged
+ *   y        [T*B] rows of stride ldy, a row holding [D][H]
+ *   states   avc_gated_recurrence_states() floats, kept for the backward (NULL when there is none)
+ * T >= 1.  The backward takes dy [T*B] rows and dhT [D][B][H] (NULL = 0) and writes dgates ([D][3][H]
+ * per row, every row) and dh0 [D][B][H] (may be NULL).
+ * _step: one frame of every row, gates [B] rows [3][H], h -> h_out (h_out = h is allowed), y [B] rows. */
+size_t avc_gated_recurrence_states(int T, int B, int H, int dirs);
+size_t avc_gated_recurrence_workspace(int dtype, int T, int B, int H, int dirs);
+int avc_gated_recurrence_forward(int dtype, int T, int B, int H, int dirs, const void* gates, long ldg,
+                                 const float* h0, const int* lengths, void* y, long ldy, float* hT, float* states,
+                                 void* workspace, size_t workspace_bytes, void* stream);
+int avc_gated_recurrence_backward(int dtype, int T, int B, int H, int dirs, const void* gates, long ldg,
+                                  const int* lengths, const float* states, const void* dy, long lddy,
+                                  const float* dhT, void* dgates, long lddg, float* dh0, void* workspace,
+                                  size_t workspace_bytes, void* stream);
+int avc_gated_recurrence_step(int dtype, int B, int H, const void* gates, long ldg, const float* h, float* h_out,
+                              void* y, long ldy, void* stream);
+
+/* Log-probabilities of given classes under rows of logits (the vocoder's RAW classes,
+ * wavernn/model.py:310-317), with the rows' entropy and their `top` most probable classes.
+ *   logits   [N] rows of V, stride ldz; -inf rules a class out
+ *   tokens   [N]: the class of each row.  ignore_index gives log-probability 0 and no gradient through it;
+ *            any other value outside 0 .. V-1 gives NaN, and NaN through dlogp in the row's gradient
+ *   logp, entropy [N]; stats [N][3] kept for the backward (row maximum m, sum of exp(z - m), entropy)
+ *   top_logp, top_ids [N][top], top in 0 .. min(32, V): log-probabilities and classes, most probable
+ *            first, equal ones by the lower class; a NaN logit ranks as -inf
+ * A row in which every class is ruled out has log-probability -inf (top_logp too), entropy 0 and gradient 0.
+ * Backward: dlogits = dlogp (onehot - p) - dentropy p (log p + entropy); dlogp / dentropy [N] may be NULL (0). */
+size_t avc_token_log_probs_workspace(int dtype, long N, long V, int top);
+int avc_token_log_probs_forward(int dtype, long N, long V, const void* logits, long ldz, const long long* tokens,
+                                long long ignore_index, int top, float* logp, float* entropy, float* stats,
+                                float* top_logp, long long* top_ids, void* workspace, size_t workspace_bytes,
+                                void* stream);
+int avc_token_log_probs_backward(int dtype, long N, long V, const void* logits, long ldz, const long long* tokens,
+                                 long long ignore_index, const float* stats, const float* dlogp,
+                                 const float* dentropy, void* dlogits, long lddz, void* stream);
+
+/* Dropout from a counter-based stream; the mask is never stored: y = residual + x keep / (1 - p).
+ * Element i = row * cols + col keeps its value if the i-th 32-bit word of the stream is >= p 2^32:
+ *   key = mix(mix(mix(rng[0] + G) + rng[1]) + layer),  words 2j, 2j+1 = low, high half of mix(key + (j+1) G)
+ * with G = 0x9E3779B97F4A7C15 and mix the 64-bit finaliser of the vocoder's sampling stream.
+ *   rng   two 64-bit device words: the seed and a step count that the caller advances (so a captured
+ *         launch draws a new mask on every replay); `layer` tells the dropouts of one step apart
+ *   x, y (, residual or NULL) rows of cols.  The gradient of x is the same call on the gradient of y,
+ *         without the residual. */
+int avc_dropout(int dtype, long rows, long cols, const void* x, long ldx, const void* residual, long ldr, double p,
+                const long long* rng, unsigned layer, void* y, long ldy, void* stream);
 
 #ifdef __cplusplus
 }
