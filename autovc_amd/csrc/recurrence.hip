@@ -11,16 +11,19 @@
 // h is formed again from states that the forward keeps every kStateStep frames.
 //
 // Everything but the loaded and stored elements is fp32.  1 - f is never formed by subtraction.
+#include <algorithm>
+#include <type_traits>
+
 #include "typed.h"
 
 namespace avc {
 namespace {
 
 constexpr int kStateStep = 64;  // frames between the states that the forward keeps for the backward
-constexpr int kS = 8;           // frames of a wave's stretch, all in registers
+constexpr int kSF = 8;          // frames of a wave's stretch, all in registers (forward)
+constexpr int kSB = 8;          // ... (backward)
 constexpr int kW = 8;           // waves of a workgroup = stretches of its chunk
-constexpr int kChunk = kS * kW;
-static_assert(kStateStep % kS == 0, "a kept state is the state before some wave's stretch");
+static_assert(kStateStep % kSF == 0 && kSB * kW % kStateStep == 0, "a kept state is the state before a stretch");
 
 struct RecArgs {
   int T, B, H, dirs;
@@ -68,93 +71,169 @@ __device__ __forceinline__ float candidate(float x) {
 // Where a lane works: VEC channels of one row b in one direction.  Rows narrower than a wave share
 // it.  The last vector of a row is moved back to end at H (channels that two lanes share get the
 // same value twice), so no vector is cut; lanes past the row or the batch repeat its last place
-// and store nothing.
+// and store nothing.  Frames are the same for the whole wave: an address is a scalar one for the
+// frame plus the lane's 32-bit offset in it.
 template <typename E, int VEC>
 struct Place {
-  int b, j, d, len;
+  int wave, lane, row0, lr, j, d, len;
   bool ok, rev;
   __device__ explicit Place(const RecArgs& a) {
-    const int lane = threadIdx.x & 63, g = 1 << a.log_g;
+    wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    lane = threadIdx.x & 63;
+    const int g = 1 << a.log_g;
     const int cv = (blockIdx.x % a.nct) * g + (lane & (g - 1));
-    const int row = (int)(blockIdx.x / a.nct) * (64 >> a.log_g) + (lane >> a.log_g);
-    ok = cv * VEC < a.H && row < a.B;
+    row0 = (int)(blockIdx.x / a.nct) * (64 >> a.log_g);
+    lr = lane >> a.log_g;
+    ok = cv * VEC < a.H && row0 + lr < a.B;
     j = min(cv * VEC, a.H - VEC);
-    b = min(row, a.B - 1);
+    lr = min(lr, a.B - 1 - row0);
     d = blockIdx.z;
     rev = a.dirs == 2 || d == 1;
-    len = a.lengths ? min(max(a.lengths[b], 0), a.T) : a.T;
+    len = a.lengths ? min(max(a.lengths[row0 + lr], 0), a.T) : a.T;
   }
-  __device__ long state(const RecArgs& a) const { return ((long)d * a.B + b) * a.H + j; }
+  // a matrix of frame rows of stride ld, `width` elements a direction
+  __device__ E* rows(const void* p, long ld, int width) const {
+    return static_cast<E*>(const_cast<void*>(p)) + (long)row0 * ld + (long)d * width;
+  }
+  __device__ unsigned off(long ld) const { return (unsigned)lr * (unsigned)ld + (unsigned)j; }
+  // the state of [D][B][H] floats
+  __device__ long state0(const RecArgs& a) const { return ((long)d * a.B + row0) * a.H; }
 };
+template <int VEC, typename E>
+__device__ __forceinline__ Vec<E, VEC> take(const E* scalar, unsigned off) {
+  return vload<E, VEC>(reinterpret_cast<const E*>(reinterpret_cast<const char*>(scalar) + off * (unsigned)sizeof(E)));
+}
+template <int VEC, typename E>
+__device__ __forceinline__ void give(E* scalar, unsigned off, const float (&x)[VEC]) {
+  vstore<E, VEC>(reinterpret_cast<E*>(reinterpret_cast<char*>(scalar) + off * (unsigned)sizeof(E)), x);
+}
+template <int VEC>
+__device__ __forceinline__ void take_to(float (&x)[VEC], const float* scalar, unsigned off) {
+  const Vec<float, VEC> r = take<VEC>(scalar, off);
+#pragma unroll
+  for (int v = 0; v < VEC; ++v) x[v] = r.v[v];
+}
 
-// frame of step s (0 .. T-1 in the direction's own order), and whether it is inside the sequence;
-// the frame is one that exists, also where it is not live
+// frame of step s of a direction's own order (s < T)
+__device__ __forceinline__ int frame_of(const RecArgs& a, int s, bool rev) { return rev ? a.T - 1 - s : s; }
+// What of the S frames from step s0 is live for the wave: nothing, everything for every lane, or a part
+enum Live { kNone, kPart, kAll };
+template <bool RAGGED, int S>
+__device__ __forceinline__ Live live_of(const RecArgs& a, int s0, bool rev, int len) {
+  if (s0 >= a.T) return kNone;
+  if (!RAGGED) return s0 + S <= a.T ? kAll : kPart;
+  const int t0 = rev ? max(a.T - s0 - S, 0) : s0, t1 = rev ? a.T - s0 : min(s0 + S, a.T);
+  if (!__any(t0 < len)) return kNone;
+  return s0 + S <= a.T && __all(t1 <= len) ? kAll : kPart;
+}
 template <bool RAGGED>
-__device__ __forceinline__ int frame_of(const RecArgs& a, int s, bool rev, int len, bool& live) {
-  const int sc = min(s, a.T - 1);
-  const int t = rev ? a.T - 1 - sc : sc;
-  live = s < a.T && (!RAGGED || t < len);
-  return RAGGED ? min(t, max(len - 1, 0)) : t;
+__device__ __forceinline__ bool is_live(const RecArgs& a, int s, bool rev, int len) {
+  return s < a.T && (!RAGGED || frame_of(a, s, rev) < len);
+}
+
+// A gate that is not read: f = 1 and 1 - f = 0 (kept), z = 0, o = 0
+template <typename E, int VEC>
+__device__ __forceinline__ Vec<E, VEC> constant(float x) {
+  Vec<E, VEC> r;
+#pragma unroll
+  for (int v = 0; v < VEC; ++v) r.v[v] = static_cast<E>(x);
+  return r;
+}
+
+// Carries x through the segments lo .. hi-1 (BACK: from the last to the first): the waves join a
+// run of segments each, side by side, and every wave then joins the runs.
+template <int VEC, bool BACK>
+__device__ void join_segments(const RecArgs& a, int lo, int hi, const float* agg, unsigned off, long nstate, int wave,
+                              int lane, float (*part)[2 + BACK][64][VEC], float (&x)[VEC]) {
+  if (lo >= hi) return;
+  const int per = (hi - lo + kW - 1) / kW;
+  float A[VEC], Bv[VEC];
+#pragma unroll
+  for (int v = 0; v < VEC; ++v) A[v] = 1.0f, Bv[v] = 0.0f;
+  const int q0 = lo + wave * per, q1 = min(q0 + per, hi);
+#pragma unroll 4
+  for (int i = q0; i < q1; ++i) {
+    const float* p = agg + (long)(BACK ? q0 + q1 - 1 - i : i) * 2 * nstate;
+    float pa[VEC], pb[VEC];
+    take_to<VEC>(pa, p, off);
+    take_to<VEC>(pb, p + nstate, off);
+#pragma unroll
+    for (int v = 0; v < VEC; ++v) {
+      Bv[v] = fmaf(pa[v], Bv[v], pb[v]);
+      A[v] *= pa[v];
+    }
+  }
+#pragma unroll
+  for (int v = 0; v < VEC; ++v) part[wave][0][lane][v] = A[v], part[wave][1][lane][v] = Bv[v];
+  __syncthreads();
+#pragma unroll
+  for (int ww = 0; ww < kW; ++ww) {
+    const int w = BACK ? kW - 1 - ww : ww;
+#pragma unroll
+    for (int v = 0; v < VEC; ++v) x[v] = fmaf(part[w][0][lane][v], x[v], part[w][1][lane][v]);
+  }
+  __syncthreads();
 }
 
 template <typename E, int VEC, bool RAGGED>
-__global__ __launch_bounds__(kW * 64) void recurrence_forward_kernel(RecArgs a) {
+__global__ __launch_bounds__(kW * 64, 4) void recurrence_forward_kernel(RecArgs a) {
+  constexpr int kS = kSF, kChunk = kS * kW;
   const Place<E, VEC> at(a);
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  const int wave = at.wave, lane = at.lane;
   __shared__ float part[2][kW][2][64][VEC];
-  const E* g = static_cast<const E*>(a.gates) + (long)at.b * a.ldg + (long)at.d * 3 * a.H + at.j;
-  E* y = static_cast<E*>(a.y) + (long)at.b * a.ldy + (long)at.d * a.H + at.j;
+  const E* g = at.rows(a.gates, a.ldg, 3 * a.H);
+  E* y = at.rows(a.y, a.ldy, a.H);
+  const unsigned goff = at.off(a.ldg), yoff = at.off(a.ldy), soff = at.off(a.H);
   const long gstep = (long)a.B * a.ldg, ystep = (long)a.B * a.ldy;
-  const long st = at.state(a), nstate = (long)(a.dirs == 3 ? 2 : 1) * a.B * a.H;
+  const long st0 = at.state0(a), nstate = (long)(a.dirs == 3 ? 2 : 1) * a.B * a.H;
 
-  float h[VEC];
-#pragma unroll
-  for (int v = 0; v < VEC; ++v) h[v] = a.h0 ? a.h0[st + v] : 0.0f;
-  for (int q = 0; q < (int)blockIdx.y; ++q) {  // the segments before this one, in order
-    const float* p = a.agg + (long)q * 2 * nstate + st;
-#pragma unroll
-    for (int v = 0; v < VEC; ++v) h[v] = fmaf(p[v], h[v], p[nstate + v]);
-  }
-
+  float h[VEC] = {};
+  if (a.h0) take_to<VEC>(h, a.h0 + st0, soff);
   const int first = blockIdx.y * a.seg_chunks;
   const int last = min(first + a.seg_chunks, (a.T + kChunk - 1) / kChunk);
   Vec<E, VEC> rf[kS], rc[kS], ro[kS];
   auto load = [&](int chunk) {
     const int s0 = chunk * kChunk + wave * kS;
-    if (chunk >= last || s0 >= a.T) return;
+    if (chunk >= last) return;
+    auto frame = [&](int k) {
+      const E* p = g + frame_of(a, s0 + k, at.rev) * gstep;
+      rf[k] = take<VEC>(p, goff);
+      rc[k] = take<VEC>(p + a.H, goff);
+      ro[k] = take<VEC>(p + 2 * a.H, goff);
+    };
+    const Live live = live_of<RAGGED, kS>(a, s0, at.rev, at.len);
+    if (live == kAll) {
 #pragma unroll
-    for (int k = 0; k < kS; ++k) {
-      bool live;
-      const E* p = g + frame_of<RAGGED>(a, s0 + k, at.rev, at.len, live) * gstep;
-      rf[k] = vload<E, VEC>(p);
-      rc[k] = vload<E, VEC>(p + a.H);
-      ro[k] = vload<E, VEC>(p + 2 * a.H);
+      for (int k = 0; k < kS; ++k) frame(k);
+    } else if (live == kPart) {
+#pragma unroll
+      for (int k = 0; k < kS; ++k) {
+        rf[k] = constant<E, VEC>(INFINITY), rc[k] = constant<E, VEC>(0.0f), ro[k] = constant<E, VEC>(-INFINITY);
+        if (is_live<RAGGED>(a, s0 + k, at.rev, at.len)) frame(k);
+      }
     }
   };
   load(first);
+  join_segments<VEC, false>(a, 0, blockIdx.y, a.agg + st0, soff, nstate, wave, lane, part[first & 1], h);
   for (int chunk = first; chunk < last; ++chunk) {
     const int s0 = chunk * kChunk + wave * kS;
+    const Live live = live_of<RAGGED, kS>(a, s0, at.rev, at.len);
     float prod[kS][VEC], loc[kS][VEC], o[kS][VEC];
     float A[VEC], Bv[VEC];
 #pragma unroll
     for (int v = 0; v < VEC; ++v) A[v] = 1.0f, Bv[v] = 0.0f;
-    if (s0 < a.T) {
+    if (live != kNone) {
 #pragma unroll
-      for (int k = 0; k < kS; ++k) {
-        bool live;
-        frame_of<RAGGED>(a, s0 + k, at.rev, at.len, live);
+      for (int k = 0; k < kS; ++k)
 #pragma unroll
         for (int v = 0; v < VEC; ++v) {
           float f, i;
           forget_gate((float)rf[k].v[v], f, i);
           const float z = candidate<E>((float)rc[k].v[v]);
           o[k][v] = gate_sigmoid((float)ro[k].v[v]);
-          Bv[v] = live ? fmaf(f, Bv[v], i * z) : Bv[v];
-          A[v] = live ? A[v] * f : A[v];
-          prod[k][v] = A[v];
-          loc[k][v] = Bv[v];
+          loc[k][v] = Bv[v] = fmaf(f, Bv[v], i * z);
+          prod[k][v] = A[v] *= f;
         }
-      }
     }
     float (*mine)[2][64][VEC] = part[chunk & 1];
 #pragma unroll
@@ -170,112 +249,99 @@ __global__ __launch_bounds__(kW * 64) void recurrence_forward_kernel(RecArgs a) 
         h[v] = fmaf(mine[w][0][lane][v], h[v], mine[w][1][lane][v]);
       }
     }
-    if (s0 < a.T && at.ok) {
-      if (a.states && s0 % kStateStep == 0) {
+    if (s0 >= a.T || !at.ok) continue;
+    if (a.states && s0 % kStateStep == 0) give<VEC>(a.states + (long)(s0 / kStateStep) * nstate + st0, soff, hin);
 #pragma unroll
-        for (int v = 0; v < VEC; ++v) a.states[(long)(s0 / kStateStep) * nstate + st + v] = hin[v];
-      }
-#pragma unroll
-      for (int k = 0; k < kS; ++k) {
-        if (s0 + k >= a.T) break;
-        const int t = at.rev ? a.T - 1 - s0 - k : s0 + k;
-        const bool live = !RAGGED || t < at.len;
+    for (int k = 0; k < kS; ++k) {
+      if (s0 + k < a.T) {
+        const int t = frame_of(a, s0 + k, at.rev);
+        const bool on = !RAGGED || t < at.len;
         float out[VEC];
 #pragma unroll
-        for (int v = 0; v < VEC; ++v) out[v] = live ? o[k][v] * fmaf(prod[k][v], hin[v], loc[k][v]) : 0.0f;
-        vstore<E, VEC>(y + t * ystep, out);
+        for (int v = 0; v < VEC; ++v) out[v] = on ? o[k][v] * fmaf(prod[k][v], hin[v], loc[k][v]) : 0.0f;
+        give<VEC>(y + t * ystep, yoff, out);
       }
     }
   }
-  if (a.hT && last == (a.T + kChunk - 1) / kChunk && wave == 0 && at.ok) {
-#pragma unroll
-    for (int v = 0; v < VEC; ++v) a.hT[st + v] = h[v];
-  }
+  if (a.hT && last == (a.T + kChunk - 1) / kChunk && wave == 0 && at.ok) give<VEC>(a.hT + st0, soff, h);
 }
 
 template <typename E, int VEC, bool RAGGED>
-__global__ __launch_bounds__(kW * 64) void recurrence_backward_kernel(RecArgs a) {
+__global__ __launch_bounds__(kW * 64, 2) void recurrence_backward_kernel(RecArgs a) {
+  constexpr int kS = kSB, kChunk = kS * kW;
   const Place<E, VEC> at(a);
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  const int wave = at.wave, lane = at.lane;
   __shared__ float part[2][kW][3][64][VEC];
-  const E* g = static_cast<const E*>(a.gates) + (long)at.b * a.ldg + (long)at.d * 3 * a.H + at.j;
-  const E* dy = static_cast<const E*>(a.dy) + (long)at.b * a.lddy + (long)at.d * a.H + at.j;
-  E* dg = static_cast<E*>(a.dgates) + (long)at.b * a.lddg + (long)at.d * 3 * a.H + at.j;
+  const E* g = at.rows(a.gates, a.ldg, 3 * a.H);
+  const E* dy = at.rows(a.dy, a.lddy, a.H);
+  E* dg = at.rows(a.dgates, a.lddg, 3 * a.H);
+  const unsigned goff = at.off(a.ldg), dyoff = at.off(a.lddy), dgoff = at.off(a.lddg), soff = at.off(a.H);
   const long gstep = (long)a.B * a.ldg, dystep = (long)a.B * a.lddy, dgstep = (long)a.B * a.lddg;
-  const long st = at.state(a), nstate = (long)(a.dirs == 3 ? 2 : 1) * a.B * a.H;
+  const long st0 = at.state0(a), nstate = (long)(a.dirs == 3 ? 2 : 1) * a.B * a.H;
 
-  float c[VEC];  // what the frames behind this chunk hand back
-#pragma unroll
-  for (int v = 0; v < VEC; ++v) c[v] = a.dhT ? a.dhT[st + v] : 0.0f;
-  for (int q = a.nseg - 1; q > (int)blockIdx.y; --q) {
-    const float* p = a.agg + (long)q * 2 * nstate + st;
-#pragma unroll
-    for (int v = 0; v < VEC; ++v) c[v] = fmaf(p[v], c[v], p[nstate + v]);
-  }
-
+  float c[VEC] = {};  // what the frames behind this chunk hand back
+  if (a.dhT) take_to<VEC>(c, a.dhT + st0, soff);
   const int first = blockIdx.y * a.seg_chunks;
   const int last = min(first + a.seg_chunks, (a.T + kChunk - 1) / kChunk);
   Vec<E, VEC> rf[kS], rc[kS], ro[kS], ry[kS];
   float hs[VEC];
   auto load = [&](int chunk) {
-    const int s0 = chunk * kChunk + wave * kS;
     if (chunk < first) return;
-#pragma unroll
-    for (int v = 0; v < VEC; ++v) hs[v] = a.states[(long)(chunk * (kChunk / kStateStep)) * nstate + st + v];
-    if (s0 >= a.T) return;
-#pragma unroll
-    for (int k = 0; k < kS; ++k) {
-      bool live;
-      const int t = frame_of<RAGGED>(a, s0 + k, at.rev, at.len, live);
+    const int s0 = chunk * kChunk + wave * kS;
+    const Live live = live_of<RAGGED, kS>(a, s0, at.rev, at.len);
+    if (live == kNone) return;
+    take_to<VEC>(hs, a.states + (long)(chunk * (kChunk / kStateStep)) * nstate + st0, soff);
+    auto frame = [&](int k) {
+      const int t = frame_of(a, s0 + k, at.rev);
       const E* p = g + t * gstep;
-      rf[k] = vload<E, VEC>(p);
-      rc[k] = vload<E, VEC>(p + a.H);
-      ro[k] = vload<E, VEC>(p + 2 * a.H);
-      ry[k] = vload<E, VEC>(dy + t * dystep);
+      rf[k] = take<VEC>(p, goff);
+      rc[k] = take<VEC>(p + a.H, goff);
+      ro[k] = take<VEC>(p + 2 * a.H, goff);
+      ry[k] = take<VEC>(dy + t * dystep, dyoff);
+    };
+    if (live == kAll) {
+#pragma unroll
+      for (int k = 0; k < kS; ++k) frame(k);
+    } else {
+      // a frame behind the end keeps the state and hands every gradient through
+#pragma unroll
+      for (int k = 0; k < kS; ++k) {
+        rf[k] = constant<E, VEC>(INFINITY), rc[k] = constant<E, VEC>(0.0f), ro[k] = constant<E, VEC>(-INFINITY);
+        ry[k] = constant<E, VEC>(0.0f);
+        if (is_live<RAGGED>(a, s0 + k, at.rev, at.len)) frame(k);
+      }
     }
   };
   load(last - 1);
+  join_segments<VEC, true>(a, blockIdx.y + 1, a.nseg, a.agg + st0, soff, nstate, wave, lane, part[last & 1], c);
   for (int chunk = last - 1; chunk >= first; --chunk) {
     const int s0 = chunk * kChunk + wave * kS;
+    const Live live = live_of<RAGGED, kS>(a, s0, at.rev, at.len);
     float f[kS][VEC], i[kS][VEC], z[kS][VEC], o[kS][VEC], d[kS][VEC];
-    float A[VEC], Bv[VEC], Cv[VEC];
+    float A[VEC], Bv[VEC], Cv[VEC], hin[VEC], cin[VEC];
 #pragma unroll
-    for (int v = 0; v < VEC; ++v) A[v] = 1.0f, Bv[v] = 0.0f, Cv[v] = 0.0f;
-    if (s0 < a.T) {
+    for (int v = 0; v < VEC; ++v) A[v] = 1.0f, Bv[v] = 0.0f, Cv[v] = 0.0f, hin[v] = hs[v];
+    if (live != kNone) {
 #pragma unroll
-      for (int k = 0; k < kS; ++k) {
-        bool live;
-        frame_of<RAGGED>(a, s0 + k, at.rev, at.len, live);
+      for (int k = 0; k < kS; ++k)
 #pragma unroll
         for (int v = 0; v < VEC; ++v) {
-          // a frame behind the end keeps the state and hands every gradient through
           forget_gate((float)rf[k].v[v], f[k][v], i[k][v]);
           z[k][v] = candidate<E>((float)rc[k].v[v]);
           o[k][v] = gate_sigmoid((float)ro[k].v[v]);
           d[k][v] = (float)ry[k].v[v];
-          if (RAGGED || k > 0) {
-            f[k][v] = live ? f[k][v] : 1.0f;
-            i[k][v] = live ? i[k][v] : 0.0f;
-            z[k][v] = live ? z[k][v] : 0.0f;
-            o[k][v] = live ? o[k][v] : 0.0f;
-            d[k][v] = live ? d[k][v] : 0.0f;
-          }
           Bv[v] = fmaf(f[k][v], Bv[v], i[k][v] * z[k][v]);
           A[v] *= f[k][v];
         }
-      }
 #pragma unroll
       for (int k = kS - 1; k >= 0; --k)
 #pragma unroll
         for (int v = 0; v < VEC; ++v) Cv[v] = f[k][v] * fmaf(o[k][v], d[k][v], Cv[v]);
     }
     float (*mine)[3][64][VEC] = part[chunk & 1];
-    float hin[VEC], cin[VEC];
 #pragma unroll
-    for (int v = 0; v < VEC; ++v) {
+    for (int v = 0; v < VEC; ++v)
       mine[wave][0][lane][v] = A[v], mine[wave][1][lane][v] = Bv[v], mine[wave][2][lane][v] = Cv[v];
-      hin[v] = hs[v];
-    }
     load(chunk - 1);
     __syncthreads();
 #pragma unroll
@@ -290,52 +356,68 @@ __global__ __launch_bounds__(kW * 64) void recurrence_backward_kernel(RecArgs a)
         if (w == wave) cin[v] = c[v];
         c[v] = fmaf(mine[w][0][lane][v], c[v], mine[w][2][lane][v]);
       }
-    if (s0 < a.T && at.ok) {
-      float h[kS + 1][VEC];
+    if (s0 >= a.T || !at.ok) continue;
+    if (live == kNone) {
+      // nothing but frames behind the ends of their sequences: no gradient
 #pragma unroll
-      for (int v = 0; v < VEC; ++v) h[0][v] = hin[v];
-#pragma unroll
-      for (int k = 0; k < kS; ++k)
-#pragma unroll
-        for (int v = 0; v < VEC; ++v) h[k + 1][v] = fmaf(f[k][v], h[k][v], i[k][v] * z[k][v]);
-#pragma unroll
-      for (int k = kS - 1; k >= 0; --k) {
-        float df[VEC], dc[VEC], dov[VEC];
-#pragma unroll
-        for (int v = 0; v < VEC; ++v) {
-          const float e = fmaf(o[k][v], d[k][v], cin[v]);
-          cin[v] = f[k][v] * e;
-          df[v] = cin[v] * i[k][v] * (h[k][v] - z[k][v]);
-          dc[v] = e * i[k][v] * fmaf(-z[k][v], z[k][v], 1.0f);
-          dov[v] = d[k][v] * h[k + 1][v] * fmaf(-o[k][v], o[k][v], o[k][v]);
-        }
+      for (int k = 0; k < kS; ++k) {
+        const float none[VEC] = {};
         if (s0 + k < a.T) {
-          const int t = at.rev ? a.T - 1 - s0 - k : s0 + k;
-          E* p = dg + t * dgstep;
-          vstore<E, VEC>(p, df);
-          vstore<E, VEC>(p + a.H, dc);
-          vstore<E, VEC>(p + 2 * a.H, dov);
+          E* p = dg + frame_of(a, s0 + k, at.rev) * dgstep;
+          give<VEC>(p, dgoff, none);
+          give<VEC>(p + a.H, dgoff, none);
+          give<VEC>(p + 2 * a.H, dgoff, none);
         }
+      }
+      continue;
+    }
+    float h[kS + 1][VEC];
+#pragma unroll
+    for (int v = 0; v < VEC; ++v) h[0][v] = hin[v];
+#pragma unroll
+    for (int k = 0; k < kS; ++k)
+#pragma unroll
+      for (int v = 0; v < VEC; ++v) h[k + 1][v] = fmaf(f[k][v], h[k][v], i[k][v] * z[k][v]);
+#pragma unroll
+    for (int k = kS - 1; k >= 0; --k) {
+      float df[VEC], dc[VEC], dov[VEC];
+#pragma unroll
+      for (int v = 0; v < VEC; ++v) {
+        const float e = fmaf(o[k][v], d[k][v], cin[v]);
+        cin[v] = f[k][v] * e;
+        df[v] = cin[v] * i[k][v] * (h[k][v] - z[k][v]);
+        dc[v] = e * i[k][v] * fmaf(-z[k][v], z[k][v], 1.0f);
+        dov[v] = d[k][v] * h[k + 1][v] * fmaf(-o[k][v], o[k][v], o[k][v]);
+      }
+      if (s0 + k < a.T) {
+        const int t = frame_of(a, s0 + k, at.rev);
+        E* p = dg + t * dgstep;
+        if (RAGGED && t >= at.len) {  // also where the state or a gradient is not finite
+#pragma unroll
+          for (int v = 0; v < VEC; ++v) df[v] = dc[v] = dov[v] = 0.0f;
+        }
+        give<VEC>(p, dgoff, df);
+        give<VEC>(p + a.H, dgoff, dc);
+        give<VEC>(p + 2 * a.H, dgoff, dov);
       }
     }
   }
-  if (a.dh0 && first == 0 && wave == 0 && at.ok) {
-#pragma unroll
-    for (int v = 0; v < VEC; ++v) a.dh0[st + v] = c[v];
-  }
+  if (a.dh0 && first == 0 && wave == 0 && at.ok) give<VEC>(a.dh0 + st0, soff, c);
 }
 
 // What one segment of time does to the state before it (BACK: to the gradient behind it): each
-// wave walks a run of chunks' stretches of its own, then the waves' runs are joined in order.
+// wave walks a run of stretches of its own, then the waves' runs are joined in order.
 template <typename E, int VEC, bool RAGGED, bool BACK>
 __global__ __launch_bounds__(kW * 64) void recurrence_segment_kernel(RecArgs a) {
+  constexpr int kS = BACK ? kSB : kSF;
   const Place<E, VEC> at(a);
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  const int wave = at.wave, lane = at.lane;
   __shared__ float part[kW][2][64][VEC];
-  const E* g = static_cast<const E*>(a.gates) + (long)at.b * a.ldg + (long)at.d * 3 * a.H + at.j;
-  const E* dy = BACK ? static_cast<const E*>(a.dy) + (long)at.b * a.lddy + (long)at.d * a.H + at.j : nullptr;
+  const E* g = at.rows(a.gates, a.ldg, 3 * a.H);
+  const E* dy = BACK ? at.rows(a.dy, a.lddy, a.H) : nullptr;
+  const unsigned goff = at.off(a.ldg), dyoff = at.off(a.lddy), soff = at.off(a.H);
   const long gstep = (long)a.B * a.ldg, dystep = (long)a.B * a.lddy;
-  const long st = at.state(a), nstate = (long)(a.dirs == 3 ? 2 : 1) * a.B * a.H;
+  const long st0 = at.state0(a), nstate = (long)(a.dirs == 3 ? 2 : 1) * a.B * a.H;
   // seg_chunks chunks of kW stretches: seg_chunks stretches in a row for each wave
   const int n = a.seg_chunks;
   const int base = ((int)blockIdx.y * n * kW + wave * n) * kS;
@@ -345,51 +427,55 @@ __global__ __launch_bounds__(kW * 64) void recurrence_segment_kernel(RecArgs a) 
   Vec<E, VEC> r0[kS], r1[kS], r2[kS];
   auto load = [&](int q) {
     const int s0 = base + (BACK ? n - 1 - q : q) * kS;
-    if (q >= n || s0 >= a.T) return;
-#pragma unroll
-    for (int k = 0; k < kS; ++k) {
-      bool live;
-      const int t = frame_of<RAGGED>(a, s0 + k, at.rev, at.len, live);
+    if (q >= n) return;
+    auto frame = [&](int k) {
+      const int t = frame_of(a, s0 + k, at.rev);
       const E* p = g + t * gstep;
-      r0[k] = vload<E, VEC>(p);
+      r0[k] = take<VEC>(p, goff);
       if (BACK) {
-        r1[k] = vload<E, VEC>(p + 2 * a.H);
-        r2[k] = vload<E, VEC>(dy + t * dystep);
+        r1[k] = take<VEC>(p + 2 * a.H, goff);
+        r2[k] = take<VEC>(dy + t * dystep, dyoff);
       } else {
-        r1[k] = vload<E, VEC>(p + a.H);
+        r1[k] = take<VEC>(p + a.H, goff);
+      }
+    };
+    const Live live = live_of<RAGGED, kS>(a, s0, at.rev, at.len);
+    if (live == kAll) {
+#pragma unroll
+      for (int k = 0; k < kS; ++k) frame(k);
+    } else if (live == kPart) {
+#pragma unroll
+      for (int k = 0; k < kS; ++k) {
+        r0[k] = constant<E, VEC>(INFINITY), r1[k] = r2[k] = constant<E, VEC>(0.0f);
+        if (is_live<RAGGED>(a, s0 + k, at.rev, at.len)) frame(k);
       }
     }
   };
   load(0);
   for (int q = 0; q < n; ++q) {
     const int s0 = base + (BACK ? n - 1 - q : q) * kS;
+    const Live live = live_of<RAGGED, kS>(a, s0, at.rev, at.len);
     float f[kS][VEC], u[kS][VEC];
-    if (s0 < a.T) {
+    if (live != kNone) {
 #pragma unroll
-      for (int k = 0; k < kS; ++k) {
-        bool live;
-        frame_of<RAGGED>(a, s0 + k, at.rev, at.len, live);
+      for (int k = 0; k < kS; ++k)
 #pragma unroll
         for (int v = 0; v < VEC; ++v) {
           float i;
           forget_gate((float)r0[k].v[v], f[k][v], i);
           u[k][v] = BACK ? gate_sigmoid((float)r1[k].v[v]) * (float)r2[k].v[v]
                          : i * candidate<E>((float)r1[k].v[v]);
-          f[k][v] = live ? f[k][v] : 1.0f;
-          u[k][v] = live ? u[k][v] : 0.0f;
         }
-      }
     }
     load(q + 1);
-    if (s0 < a.T) {
+    if (live == kNone) continue;
 #pragma unroll
-      for (int kk = 0; kk < kS; ++kk) {
-        const int k = BACK ? kS - 1 - kk : kk;
+    for (int kk = 0; kk < kS; ++kk) {
+      const int k = BACK ? kS - 1 - kk : kk;
 #pragma unroll
-        for (int v = 0; v < VEC; ++v) {
-          Bv[v] = BACK ? f[k][v] * (u[k][v] + Bv[v]) : fmaf(f[k][v], Bv[v], u[k][v]);
-          A[v] *= f[k][v];
-        }
+      for (int v = 0; v < VEC; ++v) {
+        Bv[v] = BACK ? f[k][v] * (u[k][v] + Bv[v]) : fmaf(f[k][v], Bv[v], u[k][v]);
+        A[v] *= f[k][v];
       }
     }
   }
@@ -397,19 +483,20 @@ __global__ __launch_bounds__(kW * 64) void recurrence_segment_kernel(RecArgs a) 
   for (int v = 0; v < VEC; ++v) part[wave][0][lane][v] = A[v], part[wave][1][lane][v] = Bv[v];
   __syncthreads();
   if (wave == 0 && at.ok) {
-    float* p = a.agg + (long)blockIdx.y * 2 * nstate + st;
+    float* p = a.agg + (long)blockIdx.y * 2 * nstate + st0;
+    float A2[VEC], B2[VEC];
 #pragma unroll
     for (int v = 0; v < VEC; ++v) {
-      float A2 = 1.0f, B2 = 0.0f;
+      A2[v] = 1.0f, B2[v] = 0.0f;
 #pragma unroll
       for (int ww = 0; ww < kW; ++ww) {
         const int w = BACK ? kW - 1 - ww : ww;
-        B2 = fmaf(part[w][0][lane][v], B2, part[w][1][lane][v]);
-        A2 *= part[w][0][lane][v];
+        B2[v] = fmaf(part[w][0][lane][v], B2[v], part[w][1][lane][v]);
+        A2[v] *= part[w][0][lane][v];
       }
-      p[v] = A2;
-      p[nstate + v] = B2;
     }
+    give<VEC>(p, soff, A2);
+    give<VEC>(p + nstate, soff, B2);
   }
 }
 
@@ -460,35 +547,47 @@ __global__ __launch_bounds__(256) void recurrence_step_kernel(int B, int H, cons
   }
 }
 
-template <typename E>
-constexpr int wide() { return sizeof(E) == 4 ? 2 : 4; }
+// channels of a lane
+template <typename E, bool BACK>
+constexpr int wide() { return sizeof(E) == 4 ? 1 : 2; }
 
-// Segments of time: with enough row tiles to fill the chip each workgroup walks its rows' whole
-// time; with fewer, time is cut into as many pieces as bring the grid there.
-int segments(int T, int B, int H, int D, int vec, int* seg_chunks) {
-  const int chunks = (T + kChunk - 1) / kChunk;
-  int log_g = 0;
-  while (log_g < 6 && (vec << log_g) < H) ++log_g;
-  const long tiles = (long)D * ((H + (vec << log_g) - 1) / (vec << log_g)) * ((B + (64 >> log_g) - 1) / (64 >> log_g));
-  long n = tiles >= 256 ? 1 : 512 / tiles;
-  if (n > chunks) n = chunks;
-  *seg_chunks = (int)((chunks + n - 1) / n);
-  return (chunks + *seg_chunks - 1) / *seg_chunks;
+// How a call is laid over the chip: lanes per row, row tiles, and segments of time.  With enough
+// row tiles to fill the chip each workgroup walks its rows' whole time; with fewer, time is cut
+// into as many segments as bring the grid there.
+struct Layout {
+  int log_g = 0, nct, nseg, seg_chunks;
+  long tiles;
+  Layout(int T, int B, int H, int D, int vec, int chunk) {
+    while (log_g < 6 && (vec << log_g) < H) ++log_g;
+    nct = (H + (vec << log_g) - 1) / (vec << log_g);
+    const int rows = 64 >> log_g, chunks = (T + chunk - 1) / chunk;
+    tiles = (long)nct * ((B + rows - 1) / rows);
+    long n = tiles * D >= 256 ? 1 : 512 / (tiles * D);
+    if (n > chunks) n = chunks;
+    seg_chunks = (int)((chunks + n - 1) / n);
+    nseg = (chunks + seg_chunks - 1) / seg_chunks;
+  }
+  size_t workspace(int B, int H, int D) const { return nseg > 1 ? (size_t)nseg * 2 * D * B * H * sizeof(float) : 0; }
+};
+
+template <typename E, bool BACK>
+Layout layout(int T, int B, int H, int D) {
+  const int vec = H >= wide<E, BACK>() ? wide<E, BACK>() : 1;
+  return Layout(T, B, H, D, vec, kW * (BACK ? kSB : kSF));
 }
 
 template <typename E, int VEC, bool BACK>
 int run_recurrence(RecArgs a, size_t ws_bytes, hipStream_t s) {
   const int D = a.dirs == 3 ? 2 : 1;
-  a.log_g = 0;
-  while (a.log_g < 6 && (VEC << a.log_g) < a.H) ++a.log_g;
-  a.nct = (a.H + (VEC << a.log_g) - 1) / (VEC << a.log_g);
-  const int rows = 64 >> a.log_g;
-  a.nseg = segments(a.T, a.B, a.H, D, VEC, &a.seg_chunks);
-  const size_t need = a.nseg > 1 ? (size_t)a.nseg * 2 * D * a.B * a.H * sizeof(float) : 0;
+  const Layout l = layout<E, BACK>(a.T, a.B, a.H, D);
+  a.log_g = l.log_g, a.nct = l.nct, a.nseg = l.nseg, a.seg_chunks = l.seg_chunks;
+  const size_t need = l.workspace(a.B, a.H, D);
   AVC_CHECK_ARG(ws_bytes >= need && (need == 0 || a.agg), "workspace smaller than avc_gated_recurrence_workspace");
-  const long tiles = (long)a.nct * ((a.B + rows - 1) / rows);
-  AVC_CHECK_ARG(tiles < (1L << 32) / (kW * 64), "B * H too large");
-  const dim3 grid((unsigned)tiles, a.nseg, D);
+  AVC_CHECK_ARG(l.tiles < (1L << 32) / (kW * 64), "B * H too large");
+  // the rows that share a wave are reached by 32-bit offsets from the first of them
+  const long widest = std::max(a.ldg, std::max(a.ldy, std::max(a.lddy, a.lddg)));
+  AVC_CHECK_ARG(widest < (1L << 29) >> (6 - l.log_g), "row stride too large");
+  const dim3 grid((unsigned)l.tiles, a.nseg, D);
   if (a.nseg > 1) {
     if (a.lengths) recurrence_segment_kernel<E, VEC, true, BACK><<<grid, kW * 64, 0, s>>>(a);
     else recurrence_segment_kernel<E, VEC, false, BACK><<<grid, kW * 64, 0, s>>>(a);
@@ -524,13 +623,19 @@ extern "C" size_t avc_gated_recurrence_states(int T, int B, int H, int dirs) {
   return (size_t)(T / kStateStep + (T % kStateStep != 0)) * (dirs == 3 ? 2 : 1) * B * H;
 }
 
+// enough for either direction's call
 extern "C" size_t avc_gated_recurrence_workspace(int dtype, int T, int B, int H, int dirs) {
   if (!dtype_ok(dtype) || T < 1 || B < 1 || H < 1 || dirs < 1 || dirs > 3) return 0;
   const int D = dirs == 3 ? 2 : 1;
-  const int wide_vec = dtype == AVC_DTYPE_F32 ? wide<float>() : wide<__bf16>();
-  int sc;
-  const int n = segments(T, B, H, D, H >= wide_vec ? wide_vec : 1, &sc);
-  return n > 1 ? (size_t)n * 2 * D * B * H * sizeof(float) : 0;
+  size_t n = 0;
+  with_dtype(dtype, [&](auto e) {
+    using E = decltype(e);
+    n = layout<E, false>(T, B, H, D).workspace(B, H, D);
+    const size_t m = layout<E, true>(T, B, H, D).workspace(B, H, D);
+    if (m > n) n = m;
+    return AVC_OK;
+  });
+  return n;
 }
 
 extern "C" int avc_gated_recurrence_forward(int dtype, int T, int B, int H, int dirs, const void* gates, long ldg,
@@ -547,8 +652,9 @@ extern "C" int avc_gated_recurrence_forward(int dtype, int T, int B, int H, int 
   a.y = y, a.ldy = ldy, a.hT = hT, a.states = states, a.agg = static_cast<float*>(workspace);
   return with_dtype(dtype, [&](auto e) {
     using E = decltype(e);
-    return H >= wide<E>() ? run_recurrence<E, wide<E>(), false>(a, workspace_bytes, s)
-                          : run_recurrence<E, 1, false>(a, workspace_bytes, s);
+    constexpr int V = wide<E, false>();
+    return H >= V ? run_recurrence<E, V, false>(a, workspace_bytes, s)
+                  : run_recurrence<E, 1, false>(a, workspace_bytes, s);
   });
 }
 
@@ -568,8 +674,9 @@ extern "C" int avc_gated_recurrence_backward(int dtype, int T, int B, int H, int
   a.dh0 = dh0, a.agg = static_cast<float*>(workspace);
   return with_dtype(dtype, [&](auto e) {
     using E = decltype(e);
-    return H >= wide<E>() ? run_recurrence<E, wide<E>(), true>(a, workspace_bytes, s)
-                          : run_recurrence<E, 1, true>(a, workspace_bytes, s);
+    constexpr int V = wide<E, true>();
+    return H >= V ? run_recurrence<E, V, true>(a, workspace_bytes, s)
+                  : run_recurrence<E, 1, true>(a, workspace_bytes, s);
   });
 }
 

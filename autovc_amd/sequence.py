@@ -6,6 +6,10 @@ column slices of a wider buffer (any row stride); other layouts are made contigu
 runs on the current stream of its tensors' device and allocates what it needs through torch, so it
 may be captured into a graph and used from several streams.  Public names are re-exported by
 `autovc_amd.ops`.
+
+On small tensors a call costs what the host spends on it, and a backward more than the same code
+elsewhere: it runs on a thread whose core has none of these objects in its caches.  So the common
+layouts take a short path through here.
 """
 from __future__ import annotations
 
@@ -13,12 +17,13 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from ._lib import call
+from ._lib import DTYPES
 
 MAX_TOP = 32
+_F32 = torch.float32
 
 
-def _check(t, name, like=None, dtypes=None):
+def _check(t, name, like=None, dtypes=DTYPES):
     """t is a tensor on a GPU (like's) of one of dtypes."""
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name} must be a tensor, got {type(t).__name__}")
@@ -26,84 +31,94 @@ def _check(t, name, like=None, dtypes=None):
         raise RuntimeError(f"autovc_amd runs on the GPU only (HIP kernels); {name} is a CPU tensor")
     if like is not None and t.device != like.device:
         raise ValueError(f"{name} is on {t.device}, expected {like.device}")
-    if t.dtype not in (_lib.DTYPES if dtypes is None else dtypes):
+    if t.dtype not in dtypes:
         raise TypeError(f"{name} has dtype {t.dtype}")
-    return t
 
 
 def _rows(t):
     """(tensor, row stride) of a matrix whose rows the kernels can walk: t itself unless its rows
     are not dense or overlap."""
     n, c = t.shape
+    if t.is_contiguous():
+        return t, c
     s = t.stride()
     if (c > 1 and s[1] != 1) or (n > 1 and s[0] < c):
-        t = t.contiguous()
-        s = t.stride()
+        return t.contiguous(), c
     return t, (s[0] if n > 1 else c)
 
 
-def _launch(t, name, *args):
-    """call(name, *args, stream) with t's device current."""
-    dev = t.device
+def _launch(dev, name, *args):
+    """The library's call of that name on dev's current stream, with dev current."""
     if dev.index == torch.cuda.current_device():
-        call(name, *args, _lib.stream(dev))
+        status = getattr(_lib.load(), name)(*args, _lib.stream(dev))
     else:
         with torch.cuda.device(dev):
-            call(name, *args, _lib.stream(dev))
+            status = getattr(_lib.load(), name)(*args, _lib.stream(dev))
+    if status:
+        _lib.check(status, name)
 
 
-def _p(t):
-    return None if t is None else t.data_ptr()
+def _wants_grad(a, b=None):
+    return (a.requires_grad or (b is not None and b.requires_grad)) and torch.is_grad_enabled()
 
 
-def _wants_grad(*ts):
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts)
+def _backward(grads, ctx, *d):
+    """A backward that is not differentiable itself: where a graph of it is asked for
+    (create_graph), using that graph is an error; without one, grads runs as it is."""
+    if torch.is_grad_enabled():
+        return once_differentiable(grads)(ctx, *d)
+    return grads(ctx, *d)
 
 
 # ---- gated linear recurrence --------------------------------------------------------------------
-def _recurrence_forward(gates, T, B, D, H, h0, lengths, dirs, save):
-    dt = _lib.DTYPES[gates.dtype]
-    lib = _lib.load()
+def _recurrence(gates, T, B, H, h0, lengths, dirs, save):
+    dt, dev, lib = DTYPES[gates.dtype], gates.device, _lib.load()
+    D = 2 if dirs == 3 else 1
     g, ldg = _rows(gates)
-    y = torch.empty((T * B, D * H), dtype=gates.dtype, device=gates.device)
-    hT = torch.empty((D, B, H), dtype=torch.float32, device=gates.device)
-    states = None
-    if save:
-        states = torch.empty(lib.avc_gated_recurrence_states(T, B, H, dirs), dtype=torch.float32, device=gates.device)
+    y = torch.empty((T * B, D * H), dtype=gates.dtype, device=dev)
+    hT = torch.empty((D, B, H), dtype=_F32, device=dev)
+    states = torch.empty(lib.avc_gated_recurrence_states(T, B, H, dirs), dtype=_F32, device=dev) if save else None
     wb = lib.avc_gated_recurrence_workspace(dt, T, B, H, dirs)
-    ws = torch.empty(wb, dtype=torch.uint8, device=gates.device) if wb else None
-    _launch(gates, "avc_gated_recurrence_forward", dt, T, B, H, dirs, g.data_ptr(), ldg, _p(h0), _p(lengths),
-            y.data_ptr(), D * H, hT.data_ptr(), _p(states), _p(ws), wb)
+    ws = torch.empty(wb, dtype=torch.uint8, device=dev) if wb else None
+    _launch(dev, "avc_gated_recurrence_forward", dt, T, B, H, dirs, g.data_ptr(), ldg,
+            None if h0 is None else h0.data_ptr(), None if lengths is None else lengths.data_ptr(), y.data_ptr(), D * H,
+            hT.data_ptr(), states.data_ptr() if save else None, ws.data_ptr() if wb else None, wb)
     return y, hT, states
+
+
+def _recurrence_grads(ctx, dy, dhT):
+    gates, lengths, states = ctx.saved_tensors
+    T, B, H, dirs, want_h0 = ctx.dims
+    dt, dev = DTYPES[gates.dtype], gates.device
+    D = 2 if dirs == 3 else 1
+    g, ldg = _rows(gates)
+    dy, lddy = _rows(torch.zeros((T * B, D * H), dtype=gates.dtype, device=dev) if dy is None else dy)
+    dhT = None if dhT is None else dhT.contiguous()
+    dg = torch.empty((T * B, D * 3 * H), dtype=gates.dtype, device=dev)
+    dh0 = torch.empty((D, B, H), dtype=_F32, device=dev) if want_h0 else None
+    wb = _lib.load().avc_gated_recurrence_workspace(dt, T, B, H, dirs)
+    ws = torch.empty(wb, dtype=torch.uint8, device=dev) if wb else None
+    _launch(dev, "avc_gated_recurrence_backward", dt, T, B, H, dirs, g.data_ptr(), ldg,
+            None if lengths is None else lengths.data_ptr(), states.data_ptr(), dy.data_ptr(), lddy,
+            None if dhT is None else dhT.data_ptr(), dg.data_ptr(), D * 3 * H, dh0.data_ptr() if want_h0 else None,
+            ws.data_ptr() if wb else None, wb)
+    return dg, dh0, None, None, None, None, None
 
 
 class GatedRecurrence(torch.autograd.Function):
     """Autograd of gated_recurrence; the forward keeps the state before every 64th frame."""
 
     @staticmethod
-    def forward(ctx, gates, h0, T, B, D, H, lengths, dirs):
-        y, hT, states = _recurrence_forward(gates, T, B, D, H, h0, lengths, dirs, True)
+    def forward(ctx, gates, h0, T, B, H, lengths, dirs):
+        y, hT, states = _recurrence(gates, T, B, H, h0, lengths, dirs, True)
         ctx.save_for_backward(gates, lengths, states)
-        ctx.dims = (T, B, D, H, dirs, h0 is not None)
+        ctx.dims = (T, B, H, dirs, ctx.needs_input_grad[1])
         ctx.set_materialize_grads(False)
         return y, hT
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dy, dhT):
-        gates, lengths, states = ctx.saved_tensors
-        T, B, D, H, dirs, has_h0 = ctx.dims
-        g, ldg = _rows(gates)
-        dy, lddy = _rows(torch.zeros((T * B, D * H), dtype=gates.dtype, device=gates.device) if dy is None else dy)
-        dhT = None if dhT is None else dhT.contiguous()
-        dg = torch.empty((T * B, D * 3 * H), dtype=gates.dtype, device=gates.device)
-        dh0 = torch.empty((D, B, H), dtype=torch.float32, device=gates.device) if has_h0 and ctx.needs_input_grad[1] else None
-        dt = _lib.DTYPES[gates.dtype]
-        wb = _lib.load().avc_gated_recurrence_workspace(dt, T, B, H, dirs)
-        ws = torch.empty(wb, dtype=torch.uint8, device=gates.device) if wb else None
-        _launch(gates, "avc_gated_recurrence_backward", dt, T, B, H, dirs, g.data_ptr(), ldg, _p(lengths),
-                states.data_ptr(), dy.data_ptr(), lddy, _p(dhT), dg.data_ptr(), D * 3 * H, _p(dh0), _p(ws), wb)
-        return dg, dh0, None, None, None, None, None, None
+        return _backward(_recurrence_grads, ctx, dy, dhT)
 
 
 def gated_recurrence(gates, T, B, h0=None, lengths=None, dirs=1):
@@ -126,7 +141,7 @@ def gated_recurrence(gates, T, B, h0=None, lengths=None, dirs=1):
         raise ValueError(f"gates must be [T*B = {T * B}][{3 * D} * H], got {tuple(gates.shape)}")
     H = gates.shape[1] // (3 * D)
     if h0 is not None:
-        _check(h0, "h0", gates, (torch.float32,))
+        _check(h0, "h0", gates, (_F32,))
         if tuple(h0.shape) != (D, B, H):
             raise ValueError(f"h0 must be {(D, B, H)}, got {tuple(h0.shape)}")
         h0 = h0.contiguous()
@@ -136,11 +151,11 @@ def gated_recurrence(gates, T, B, h0=None, lengths=None, dirs=1):
             raise ValueError(f"lengths must be {(B,)}, got {tuple(lengths.shape)}")
         lengths = lengths.clamp(0, T).to(torch.int32) if lengths.dtype == torch.int64 else lengths.contiguous()
     if T * B == 0:
-        hT = h0.clone() if h0 is not None else torch.zeros((D, B, H), dtype=torch.float32, device=gates.device)
+        hT = h0.clone() if h0 is not None else torch.zeros((D, B, H), dtype=_F32, device=gates.device)
         return gates[:, :D * H].contiguous(), hT
     if _wants_grad(gates, h0):
-        return GatedRecurrence.apply(gates, h0, T, B, D, H, lengths, dirs)
-    return _recurrence_forward(gates, T, B, D, H, h0, lengths, dirs, False)[:2]
+        return GatedRecurrence.apply(gates, h0, T, B, H, lengths, dirs)
+    return _recurrence(gates, T, B, H, h0, lengths, dirs, False)[:2]
 
 
 def gated_recurrence_step(gates, state, out_state=None):
@@ -148,7 +163,7 @@ def gated_recurrence_step(gates, state, out_state=None):
     state [B][H] fp32 -> (y [B][H], new state).  The new state goes to out_state (which may be
     `state` itself) or to a fresh tensor.  No autograd."""
     _check(gates, "gates")
-    _check(state, "state", gates, (torch.float32,))
+    _check(state, "state", gates, (_F32,))
     if gates.dim() != 2 or gates.shape[1] == 0 or gates.shape[1] % 3:
         raise ValueError(f"gates must be [B][3 * H], got {tuple(gates.shape)}")
     if _wants_grad(gates, state):
@@ -156,20 +171,22 @@ def gated_recurrence_step(gates, state, out_state=None):
     B, H = gates.shape[0], gates.shape[1] // 3
     if tuple(state.shape) != (B, H):
         raise ValueError(f"state must be {(B, H)}, got {tuple(state.shape)}")
+    dev = gates.device
     if out_state is None:
-        out_state = torch.empty((B, H), dtype=torch.float32, device=gates.device)
+        out_state = torch.empty((B, H), dtype=_F32, device=dev)
     else:
-        _check(out_state, "out_state", gates, (torch.float32,))
+        _check(out_state, "out_state", gates, (_F32,))
         if tuple(out_state.shape) != (B, H) or not out_state.is_contiguous():
             raise ValueError(f"out_state must be a contiguous {(B, H)}")
-        if out_state.data_ptr() != state.data_ptr() and _overlap(out_state, state):
+        if out_state is not state and _overlap(out_state, state) and not (
+                out_state.data_ptr() == state.data_ptr() and state.is_contiguous()):
             raise ValueError("out_state overlaps state without being it")
-    y = torch.empty((B, H), dtype=gates.dtype, device=gates.device)
+    y = torch.empty((B, H), dtype=gates.dtype, device=dev)
     if B:
         g, ldg = _rows(gates)
         state = state.contiguous()
-        _launch(gates, "avc_gated_recurrence_step", _lib.DTYPES[gates.dtype], B, H, g.data_ptr(), ldg,
-                state.data_ptr(), out_state.data_ptr(), y.data_ptr(), H)
+        _launch(dev, "avc_gated_recurrence_step", DTYPES[gates.dtype], B, H, g.data_ptr(), ldg, state.data_ptr(),
+                out_state.data_ptr(), y.data_ptr(), H)
     return y, out_state
 
 
@@ -181,21 +198,36 @@ def _overlap(a, b):
 
 
 # ---- log-probabilities of given classes -----------------------------------------------------------
-def _log_probs_forward(logits, tokens, top, ignore, save):
-    dt = _lib.DTYPES[logits.dtype]
-    dev = logits.device
+def _log_probs(logits, tokens, top, ignore, save):
+    dt, dev = DTYPES[logits.dtype], logits.device
     N, V = logits.shape
     z, ldz = _rows(logits)
-    logp, entropy = torch.empty((2, N), dtype=torch.float32, device=dev).unbind(0)
-    top_logp = torch.empty((N, top), dtype=torch.float32, device=dev)
+    logp = torch.empty(N, dtype=_F32, device=dev)
+    entropy = torch.empty(N, dtype=_F32, device=dev)
+    top_logp = torch.empty((N, top), dtype=_F32, device=dev)
     top_ids = torch.empty((N, top), dtype=torch.int64, device=dev)
-    stats = torch.empty((N, 3), dtype=torch.float32, device=dev) if save else None
+    stats = torch.empty((N, 3), dtype=_F32, device=dev) if save else None
     wb = _lib.load().avc_token_log_probs_workspace(dt, N, V, top)
     ws = torch.empty(wb, dtype=torch.uint8, device=dev) if wb else None
     if N:
-        _launch(logits, "avc_token_log_probs_forward", dt, N, V, z.data_ptr(), ldz, tokens.data_ptr(), ignore, top,
-                logp.data_ptr(), entropy.data_ptr(), _p(stats), top_logp.data_ptr(), top_ids.data_ptr(), _p(ws), wb)
+        _launch(dev, "avc_token_log_probs_forward", dt, N, V, z.data_ptr(), ldz, tokens.data_ptr(), ignore, top,
+                logp.data_ptr(), entropy.data_ptr(), stats.data_ptr() if save else None, top_logp.data_ptr(),
+                top_ids.data_ptr(), ws.data_ptr() if wb else None, wb)
     return logp, entropy, top_logp, top_ids, stats
+
+
+def _log_probs_grads(ctx, dlogp, dentropy, _top_logp, _top_ids):
+    logits, tokens, stats = ctx.saved_tensors
+    N, V = logits.shape
+    z, ldz = _rows(logits)
+    d = torch.empty((N, V), dtype=logits.dtype, device=logits.device)
+    dlogp = None if dlogp is None else dlogp.contiguous()
+    dentropy = None if dentropy is None else dentropy.contiguous()
+    if N:
+        _launch(logits.device, "avc_token_log_probs_backward", DTYPES[logits.dtype], N, V, z.data_ptr(), ldz,
+                tokens.data_ptr(), ctx.ignore, stats.data_ptr(), None if dlogp is None else dlogp.data_ptr(),
+                None if dentropy is None else dentropy.data_ptr(), d.data_ptr(), V)
+    return d, None, None, None
 
 
 class TokenLogProbs(torch.autograd.Function):
@@ -203,7 +235,7 @@ class TokenLogProbs(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, logits, tokens, top, ignore):
-        logp, entropy, top_logp, top_ids, stats = _log_probs_forward(logits, tokens, top, ignore, True)
+        logp, entropy, top_logp, top_ids, stats = _log_probs(logits, tokens, top, ignore, True)
         ctx.save_for_backward(logits, tokens, stats)
         ctx.ignore = ignore
         ctx.mark_non_differentiable(top_logp, top_ids)
@@ -211,18 +243,8 @@ class TokenLogProbs(torch.autograd.Function):
         return logp, entropy, top_logp, top_ids
 
     @staticmethod
-    @once_differentiable
-    def backward(ctx, dlogp, dentropy, _top_logp, _top_ids):
-        logits, tokens, stats = ctx.saved_tensors
-        N, V = logits.shape
-        z, ldz = _rows(logits)
-        d = torch.empty((N, V), dtype=logits.dtype, device=logits.device)
-        dlogp = None if dlogp is None else dlogp.contiguous()
-        dentropy = None if dentropy is None else dentropy.contiguous()
-        if N:
-            _launch(logits, "avc_token_log_probs_backward", _lib.DTYPES[logits.dtype], N, V, z.data_ptr(), ldz,
-                    tokens.data_ptr(), ctx.ignore, stats.data_ptr(), _p(dlogp), _p(dentropy), d.data_ptr(), V)
-        return d, None, None, None
+    def backward(ctx, *d):
+        return _backward(_log_probs_grads, ctx, *d)
 
 
 def token_log_probs(logits, tokens, top=0, ignore_index=-100):
@@ -240,40 +262,51 @@ def token_log_probs(logits, tokens, top=0, ignore_index=-100):
     _check(tokens, "tokens", logits, (torch.int64, torch.int32))
     if logits.dim() < 1 or logits.shape[-1] < 1 or logits.shape[:-1] != tokens.shape:
         raise ValueError(f"logits [..., V >= 1] and tokens [...] must agree, got {tuple(logits.shape)} and {tuple(tokens.shape)}")
-    V, lead = logits.shape[-1], tokens.shape
+    V = logits.shape[-1]
     top = int(top)
     if not 0 <= top <= min(MAX_TOP, V):
         raise ValueError(f"top must be 0 .. {min(MAX_TOP, V)}, got {top}")
-    tokens = tokens.to(torch.int64).contiguous()
-    flat = logits.dim() == 2
-    if not flat:
+    if tokens.dtype != torch.int64 or not tokens.is_contiguous():
+        tokens = tokens.to(torch.int64).contiguous()
+    lead = None
+    if logits.dim() != 2:
+        lead = tokens.shape
         logits, tokens = logits.reshape(-1, V), tokens.reshape(-1)
     if _wants_grad(logits):
         out = TokenLogProbs.apply(logits, tokens, top, int(ignore_index))
     else:
-        out = _log_probs_forward(logits, tokens, top, int(ignore_index), False)[:4]
-    if flat:
+        out = _log_probs(logits, tokens, top, int(ignore_index), False)[:4]
+    if lead is None:
         return out
     return out[0].view(lead), out[1].view(lead), out[2].view(*lead, top), out[3].view(*lead, top)
 
 
 # ---- counter-based dropout --------------------------------------------------------------------------
 def _drop(x, residual, p, rng, layer):
-    shape = x.shape
-    if x.dim() != 2 or residual is not None and residual.dim() != 2:
-        c = shape[-1] if x.dim() else 1
-        x = x.reshape(-1, c) if c else x.reshape(0, 0)
-        residual = None if residual is None else residual.reshape(x.shape)
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    if x.numel():
-        x, ldx = _rows(x)
-        ldr = 0
+    if x.is_contiguous() and (residual is None or residual.is_contiguous()):
+        y = torch.empty_like(x)
+        n = c = ldx = ldr = ldy = x.numel()
+        if n == 0:
+            return y
+        n = 1
+    else:
+        y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        if x.numel() == 0:
+            return y
+        c = ldy = x.shape[-1]
+        x, ldx = _rows(x if x.dim() == 2 else x.reshape(-1, c))
+        n, ldr = x.shape[0], 0
         if residual is not None:
-            residual, ldr = _rows(residual)
-        n, c = x.shape
-        _launch(x, "avc_dropout", _lib.DTYPES[x.dtype], n, c, x.data_ptr(), ldx, _p(residual), ldr, p, rng.data_ptr(),
-                layer, y.data_ptr(), c)
-    return y.view(shape)
+            residual, ldr = _rows(residual if residual.dim() == 2 else residual.reshape(-1, c))
+    _launch(x.device, "avc_dropout", DTYPES[x.dtype], n, c, x.data_ptr(), ldx,
+            None if residual is None else residual.data_ptr(), ldr, p, rng.data_ptr(), layer, y.data_ptr(), ldy)
+    return y
+
+
+def _dropout_grads(ctx, dy):
+    (rng,) = ctx.saved_tensors
+    need_x, need_residual = ctx.needs_input_grad[:2]
+    return _drop(dy, None, ctx.p, rng, ctx.layer) if need_x else None, dy if need_residual else None, None, None, None
 
 
 class Dropout(torch.autograd.Function):
@@ -283,15 +316,12 @@ class Dropout(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, residual, p, rng, layer):
         ctx.save_for_backward(rng)
-        ctx.cfg = (p, layer)
+        ctx.p, ctx.layer = p, layer
         return _drop(x, residual, p, rng, layer)
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dy):
-        (rng,) = ctx.saved_tensors
-        dx = _drop(dy, None, ctx.cfg[0], rng, ctx.cfg[1]) if ctx.needs_input_grad[0] else None
-        return dx, dy if ctx.needs_input_grad[1] else None, None, None, None
+        return _backward(_dropout_grads, ctx, dy)
 
 
 def dropout(x, p, rng, residual=None, layer=0):
@@ -312,7 +342,7 @@ def dropout(x, p, rng, residual=None, layer=0):
         raise ValueError(f"p must be 0 <= p < 1, got {p}")
     if not 0 <= layer < 1 << 32:
         raise ValueError(f"layer must be 0 .. 2^32 - 1, got {layer}")
-    if tuple(rng.shape) != (2,) or not rng.is_contiguous():
+    if rng.dim() != 1 or rng.shape[0] != 2 or not rng.is_contiguous():
         raise ValueError(f"rng must be a contiguous [2], got {tuple(rng.shape)}")
     if residual is not None:
         _check(residual, "residual", x, (x.dtype,))
