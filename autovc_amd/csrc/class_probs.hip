@@ -10,6 +10,8 @@
 // (a class elsewhere has k classes above it), so only those slices are read again.
 // Classes are ordered by one 64-bit key, the value's bits made monotone above the complement of
 // the class number: larger values first, equal ones by the lower class, no two keys alike.
+#include <type_traits>
+
 #include "typed.h"
 
 namespace avc {
@@ -17,6 +19,7 @@ namespace {
 
 typedef unsigned long long u64;
 constexpr int kMaxTop = 32;
+constexpr int kMaxSeg = 64;  // segments of a row: lanes of the wave that joins them
 constexpr float kFar = -200.0f;  // e^-200 is 0 in fp32: keeps 0 * -inf out of the sums
 
 template <typename E>
@@ -36,10 +39,14 @@ struct ProbArgs {
   u64* part_top; // [N][nseg][top]: its classes in order, 0 behind the last
 };
 
-__device__ __forceinline__ u64 class_key(float z, long c) {
+// (never 0, which stands for no class)
+__device__ __forceinline__ unsigned value_bits(float z) {
   if (!(z > -INFINITY)) z = -INFINITY;  // a NaN ranks as -inf
   const unsigned b = __float_as_uint(z + 0.0f);  // -0 -> +0
-  return (u64)(b & 0x80000000u ? ~b : b | 0x80000000u) << 32 | (0xffffffffu - (unsigned)c);
+  return b & 0x80000000u ? ~b : b | 0x80000000u;
+}
+__device__ __forceinline__ u64 class_key(float z, long c) {
+  return (u64)value_bits(z) << 32 | (0xffffffffu - (unsigned)c);
 }
 __device__ __forceinline__ float key_value(u64 k) {
   const unsigned b = (unsigned)(k >> 32);
@@ -47,23 +54,49 @@ __device__ __forceinline__ float key_value(u64 k) {
 }
 __device__ __forceinline__ long key_class(u64 k) { return 0xffffffffu - (unsigned)k; }
 
-__device__ __forceinline__ float wave_max(float x) {
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) x = fmaxf(x, __shfl_xor(x, o));
+// Reductions over a wave by data-parallel-primitive moves (a few cycles a step, where a shuffle
+// through the LDS crossbar takes some hundred): after four shifts the last lane of each row of 16
+// holds its row, two broadcasts join the rows in lane 63.  The order is the same in every run.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ unsigned dpp_move(unsigned x, unsigned none) {
+  return (unsigned)__builtin_amdgcn_update_dpp((int)none, (int)x, CTRL, ROWS, 0xf, false);
+}
+template <typename T, typename Op, typename Step>
+__device__ __forceinline__ T dpp_reduce(T x, Op op, Step step) {
+  x = op(x, step(x, std::integral_constant<int, 0x111>{}, std::integral_constant<int, 0xf>{}));
+  x = op(x, step(x, std::integral_constant<int, 0x112>{}, std::integral_constant<int, 0xf>{}));
+  x = op(x, step(x, std::integral_constant<int, 0x114>{}, std::integral_constant<int, 0xf>{}));
+  x = op(x, step(x, std::integral_constant<int, 0x118>{}, std::integral_constant<int, 0xf>{}));
+  x = op(x, step(x, std::integral_constant<int, 0x142>{}, std::integral_constant<int, 0xa>{}));
+  x = op(x, step(x, std::integral_constant<int, 0x143>{}, std::integral_constant<int, 0xc>{}));
   return x;
+}
+__device__ __forceinline__ float last_lane(float x) {
+  return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(x), 63));
+}
+__device__ __forceinline__ float wave_max(float x) {
+  return last_lane(dpp_reduce(
+      x, [](float p, float q) { return fmaxf(p, q); },
+      [](float p, auto ctrl, auto rows) {
+        return __uint_as_float(dpp_move<ctrl.value, rows.value>(__float_as_uint(p), 0xff800000u));
+      }));
 }
 __device__ __forceinline__ float wave_sum(float x) {
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) x += __shfl_xor(x, o);
-  return x;
+  return last_lane(dpp_reduce(
+      x, [](float p, float q) { return p + q; },
+      [](float p, auto ctrl, auto rows) {
+        return __uint_as_float(dpp_move<ctrl.value, rows.value>(__float_as_uint(p), 0u));
+      }));
 }
 __device__ __forceinline__ u64 wave_max(u64 x) {
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) {
-    const u64 y = __shfl_xor(x, o);
-    x = y > x ? y : x;
-  }
-  return x;
+  x = dpp_reduce(
+      x, [](u64 p, u64 q) { return q > p ? q : p; },
+      [](u64 p, auto ctrl, auto rows) {
+        const unsigned lo = dpp_move<ctrl.value, rows.value>((unsigned)p, 0u);
+        return (u64)dpp_move<ctrl.value, rows.value>((unsigned)(p >> 32), 0u) << 32 | lo;
+      });
+  return (u64)(unsigned)__builtin_amdgcn_readlane((unsigned)(x >> 32), 63) << 32 |
+         (unsigned)__builtin_amdgcn_readlane((unsigned)x, 63);
 }
 
 struct Sums {
@@ -109,91 +142,190 @@ __device__ __forceinline__ void row_sync() {
   }
 }
 
+// The wave's k-th largest value, bit by bit (0 where fewer than k lanes are above 0).
+template <typename T>
+__device__ __forceinline__ T wave_kth(T x, int k) {
+  T least = 0;
+  for (T bit = (T)1 << (sizeof(T) * 8 - 1); bit; bit >>= 1)
+    if (__popcll(__ballot(x >= (least | bit))) >= k) least |= bit;
+  return least;
+}
+// Appends the lanes' keys for which `in` holds to a list in LDS that has room for cap: one atomic
+// a wave.  `count` goes on counting past cap.
+__device__ __forceinline__ void append(u64* list, int* count, int cap, bool in, u64 key) {
+  const u64 m = __ballot(in);
+  if (!in) return;
+  const int lane = threadIdx.x & 63, first = __ffsll(m) - 1;
+  int at = 0;
+  if (lane == first) at = atomicAdd(count, __popcll(m));
+  at = __shfl(at, first) + __popcll(m & ((1ull << lane) - 1));
+  if (at < cap) list[at] = key;
+}
+
 template <int GT>
 struct TopShared {
-  static constexpr int kCap = GT == 64 ? 192 : 1024;  // candidates that are ranked at once
-  u64 best[GT];
-  int sel[kMaxTop];
-  u64 tau;
-  int count;
+  static constexpr int kCap = GT == 64 ? 128 : 256;  // candidates that are ranked at once
   u64 cand[kCap];
+  unsigned tau;
+  int count, nsel;
+  int ties[GT / 64];
+  short sel[GT];
 };
-
-// The row segment's `k` largest keys in order, emit(rank, key).  best: the thread's largest key (0:
-// its slice is empty); key_of(t, j): the j-th key of thread t's slice, j < per (0 past its end).
-template <int GT, typename KeyOf, typename Emit>
-__device__ void select_top(TopShared<GT>& sh, int tid, int k, u64 best, int per, KeyOf key_of, Emit emit) {
-  sh.best[tid] = best;
-  if (tid == 0) sh.tau = 1, sh.count = 0;
-  row_sync<GT>();
-  int rank = 0, held = 0;
-  for (int i = 0; i < GT; ++i) {
-    const u64 o = sh.best[i];
-    rank += o > best;
-    held += o != 0;
-  }
-  if (best != 0 && rank < k) {
-    sh.sel[rank] = tid;
-    if (rank == k - 1) sh.tau = best;
-  }
-  row_sync<GT>();
-  const int nsel = min(k, held);
-  const u64 tau = sh.tau;
-  for (int i = tid; i < nsel * per; i += GT) {
-    const u64 key = key_of(sh.sel[i / per], i % per);
-    if (key >= tau) {
-      const int at = atomicAdd(&sh.count, 1);
-      if (at < TopShared<GT>::kCap) sh.cand[at] = key;
-    }
-  }
-  row_sync<GT>();
-  const int n = sh.count;
-  if (n <= TopShared<GT>::kCap) {
-    // the candidates stand in any order; their ranks do not depend on it
-    for (int i = tid; i < n; i += GT) {
-      const u64 key = sh.cand[i];
-      int r = 0;
-      for (int j = 0; j < n; ++j) r += sh.cand[j] > key;
-      if (r < k) emit(r, key);
-    }
-  } else {
-    // many large classes in few slices: one class a round
-    u64 under = ~0ull;
-    for (int r = 0; r < k; ++r) {
-      u64 mine = 0;
-      for (int i = tid; i < nsel * per; i += GT) {
-        const u64 key = key_of(sh.sel[i / per], i % per);
-        if (key < under && key > mine) mine = key;
-      }
-      mine = wave_max(mine);
-      if (GT > 64) {
-        row_sync<GT>();
-        if ((tid & 63) == 0) sh.best[tid >> 6] = mine;
-        row_sync<GT>();
-#pragma unroll
-        for (int w = 0; w < GT / 64; ++w) mine = sh.best[w] > mine ? sh.best[w] : mine;
-      }
-      under = mine;
-      if (tid == 0) emit(r, mine);
-    }
+// n keys in any order: those whose rank is below k go out with it
+template <int GT, typename Emit>
+__device__ __forceinline__ void rank_out(const u64* cand, int n, int tid, int k, Emit emit) {
+  for (int i = tid; i < n; i += GT) {
+    const u64 key = cand[i];
+    int r = 0;
+    for (int j = 0; j < n; ++j) r += cand[j] > key;
+    if (r < k) emit(r, key);
   }
 }
 
+// The `k` largest keys of classes c0 .. c1-1 in order, emit(rank, key).  mine: the largest value_bits
+// of the thread's slice (0: empty); a slice is the thread's vectors, GT vectors apart.  Only slices
+// whose largest is at least a value that k classes are known to reach can hold one of the k.
+template <typename E, int GT, typename Emit>
+__device__ void select_top(TopShared<GT>& sh, int tid, int k, unsigned mine, const E* z, long c0, long c1, Emit emit) {
+  constexpr int VEC = width<E>(), kCap = TopShared<GT>::kCap;
+  const int lane = tid & 63, wave = tid >> 6;
+  if (tid == 0) sh.tau = 1, sh.count = 0, sh.nsel = 0;
+  row_sync<GT>();
+  // k of a wave's slices reach its k-th best, so the largest of those is reached by k in all
+  const unsigned kth = wave_kth(mine, k);
+  if (lane == 0) atomicMax(&sh.tau, kth);
+  row_sync<GT>();
+  const unsigned tau = sh.tau;
+  if (mine >= tau) sh.sel[atomicAdd(&sh.nsel, 1)] = (short)tid;
+  row_sync<GT>();
+  const int nsel = sh.nsel;
+  const long rounds = (c1 - c0 + (long)GT * VEC - 1) / ((long)GT * VEC);
+  auto vector = [&](long c, float (&x)[VEC]) {
+    if (c + VEC <= c1) {
+      const Vec<E, VEC> r = vload<E, VEC>(z + c);
+#pragma unroll
+      for (int v = 0; v < VEC; ++v) x[v] = (float)r.v[v];
+    } else {
+#pragma unroll
+      for (int v = 0; v < VEC; ++v) x[v] = c + v < c1 ? (float)z[c + v] : 0.0f;
+    }
+  };
+  // 2^lg lanes a slice, a vector a lane
+  int lg = 0;
+  while (lg < 6 && (1 << lg) < rounds) ++lg;
+  auto slices = [&](auto take) {
+    for (int i = tid >> lg; i < nsel; i += GT >> lg) {
+      const int th = sh.sel[i];
+      for (long q = tid & ((1 << lg) - 1); q < rounds; q += 1 << lg) {
+        const long c = c0 + (q * GT + th) * VEC;
+        float x[VEC];
+        vector(c, x);
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) take(c + v < c1, x[v], c + v);
+      }
+    }
+  };
+  slices([&](bool in, float x, long c) {
+    append(sh.cand, &sh.count, kCap, in && value_bits(x) >= tau, class_key(x, c));
+  });
+  row_sync<GT>();
+  if (sh.count <= kCap) {
+    rank_out<GT>(sh.cand, sh.count, tid, k, emit);
+    return;
+  }
+  // More candidates than fit: classes equal to tau, as where fewer than k are not ruled out.  Those
+  // above it go first, then the lowest of the equal ones, looked for from the row's beginning.
+  row_sync<GT>();
+  if (tid == 0) sh.count = 0;
+  row_sync<GT>();
+  slices([&](bool in, float x, long c) {
+    append(sh.cand, &sh.count, kCap, in && value_bits(x) > tau, class_key(x, c));
+  });
+  row_sync<GT>();
+  const int above = sh.count;
+  if (above <= kCap - k) {
+    int have = above;
+    for (long base = c0; base < c1 && have < k; base += (long)GT * VEC) {
+      const long c = base + (long)tid * VEC;
+      float x[VEC];
+      vector(c, x);
+      int before = 0, total = 0;
+      bool tie[VEC];
+#pragma unroll
+      for (int v = 0; v < VEC; ++v) {
+        tie[v] = c + v < c1 && value_bits(x[v]) == tau;
+        const u64 m = __ballot(tie[v]);
+        before += __popcll(m & ((1ull << lane) - 1));
+        total += __popcll(m);
+      }
+      if (GT > 64) {
+        row_sync<GT>();
+        if (lane == 0) sh.ties[wave] = total;
+        row_sync<GT>();
+        total = 0;
+        for (int w = 0; w < GT / 64; ++w) {
+          if (w < wave) before += sh.ties[w];
+          total += sh.ties[w];
+        }
+      }
+      int at = have + before;
+#pragma unroll
+      for (int v = 0; v < VEC; ++v) {
+        if (tie[v]) {
+          if (at < k) sh.cand[at] = class_key(x[v], c + v);
+          ++at;
+        }
+      }
+      have += total;
+    }
+    row_sync<GT>();
+    rank_out<GT>(sh.cand, above > k ? above : have < k ? have : k, tid, k, emit);
+    return;
+  }
+  // many different large classes in few slices: one class a round
+  u64 under = ~0ull;
+  for (int r = 0; r < k; ++r) {
+    u64 most = 0;
+    slices([&](bool in, float x, long c) {
+      const u64 key = class_key(x, c);
+      if (in && key < under && key > most) most = key;
+    });
+    most = wave_max(most);
+    if (GT > 64) {
+      row_sync<GT>();
+      if (lane == 0) sh.cand[wave] = most;  // (the candidates are not used any more)
+      row_sync<GT>();
+      for (int w = 0; w < GT / 64; ++w) most = sh.cand[w] > most ? sh.cand[w] : most;
+    }
+    under = most;
+    if (tid == 0 && most != 0) emit(r, most);
+  }
+}
+
+// a row's token and its logit, asked for before the row is read
+struct Token {
+  long long tok;
+  float z;
+  template <typename E>
+  __device__ Token(const ProbArgs& a, long row, const E* logits) {
+    tok = a.tokens[row];
+    z = (float)logits[tok >= 0 && tok < a.V ? tok : 0];
+  }
+};
+
 // one thread: the row's statistics and its token's log-probability
-template <typename E>
-__device__ void finish_row(const ProbArgs& a, long row, const Sums& t) {
-  const bool empty = t.m == -INFINITY;  // (a NaN row has a NaN sum)
-  const bool none = empty && t.s == 0.0f;
+__device__ __forceinline__ void finish_row(const ProbArgs& a, long row, const Sums& t, const Token& k) {
+  // nothing left in the row (a NaN row has a NaN sum)
+  const bool none = t.m == -INFINITY && t.s == 0.0f;
   const float logs = none ? 0.0f : logf(t.s);
   const float H = none ? 0.0f : logs - t.u / t.s;
   a.entropy[row] = H;
   if (a.stats) a.stats[row * 3] = t.m, a.stats[row * 3 + 1] = t.s, a.stats[row * 3 + 2] = H;
-  const long long tok = a.tokens[row];
   float lp;
-  if (tok == a.ignore) lp = 0.0f;
-  else if (tok < 0 || tok >= a.V) lp = NAN;
+  if (k.tok == a.ignore) lp = 0.0f;
+  else if (k.tok < 0 || k.tok >= a.V) lp = NAN;
   else if (none) lp = -INFINITY;
-  else lp = ((float)static_cast<const E*>(a.z)[row * a.ldz + tok] - t.m) - logs;
+  else lp = (k.z - t.m) - logs;
   a.logp[row] = lp;
 }
 __device__ __forceinline__ void emit_top(const ProbArgs& a, long row, int r, u64 key, const Sums& t) {
@@ -203,44 +335,62 @@ __device__ __forceinline__ void emit_top(const ProbArgs& a, long row, int r, u64
   a.top_ids[row * a.top + r] = key_class(key);
 }
 
-// GT threads a row segment, 256 / GT rows a workgroup (GT = 256: blockIdx.y is the segment).
+// GT threads a row segment: a wave, four of them a workgroup, or a workgroup of 256 (blockIdx.y is
+// the segment).  A thread reads U vectors at a time and asks for the next U before it adds the first.
+template <int GT>
+constexpr int kRows = GT == 64 ? 4 : 1;  // rows of a workgroup
+
 template <typename E, int GT, bool TOP>
-__global__ __launch_bounds__(256) void class_probs_forward_kernel(ProbArgs a) {
-  constexpr int VEC = width<E>(), U = 4;
-  const int grp = threadIdx.x / GT, tid = threadIdx.x % GT;
-  const long row = (long)blockIdx.x * (256 / GT) + grp;
+__global__ __launch_bounds__(GT * kRows<GT>) void class_probs_forward_kernel(ProbArgs a) {
+  constexpr int VEC = width<E>(), U = 2;
+  constexpr long kRound = (long)GT * VEC * U;
+  const int grp = GT == 64 ? __builtin_amdgcn_readfirstlane(threadIdx.x / GT) : 0, tid = threadIdx.x % GT;
+  const long row = (long)blockIdx.x * kRows<GT> + grp;
   if (row >= a.N) return;  // a whole wave (GT = 64) or, with one row a workgroup, never
   const E* z = static_cast<const E*>(a.z) + row * a.ldz;
   const long c0 = (long)blockIdx.y * a.seg, c1 = c0 + a.seg < a.V ? c0 + a.seg : a.V;
+  const Token token(a, row, z);
   Sums t;
-  float best = -INFINITY;
-  long best_c = c0 + (long)tid * VEC;
-  for (long c = c0 + (long)tid * VEC; c < c1; c += (long)GT * VEC * U) {
-    float x[U * VEC];
+  Vec<E, VEC> r[U];
+  long c = c0;
+  auto load = [&](long from) {
+#pragma unroll
+    for (int k = 0; k < U; ++k) r[k] = vload<E, VEC>(z + from + (k * GT + tid) * VEC);
+  };
+  if (c + kRound <= c1) load(c);
+  for (; c + kRound <= c1; c += kRound) {
+    float x[U][VEC];
+#pragma unroll
+    for (int k = 0; k < U; ++k)
+#pragma unroll
+      for (int v = 0; v < VEC; ++v) x[k][v] = (float)r[k].v[v];
+    if (c + 2 * kRound <= c1) load(c + kRound);
+    t.add(reinterpret_cast<const float(&)[U * VEC]>(x));
+  }
+  if (c < c1) {  // less than a round is left, its last vector perhaps cut
+    float x[U][VEC];
 #pragma unroll
     for (int k = 0; k < U; ++k) {
-      const long ck = c + (long)k * GT * VEC;
+      const long ck = c + (k * GT + tid) * VEC;
       if (ck + VEC <= c1) {
-        const Vec<E, VEC> r = vload<E, VEC>(z + ck);
+        const Vec<E, VEC> q = vload<E, VEC>(z + ck);
 #pragma unroll
-        for (int v = 0; v < VEC; ++v) x[k * VEC + v] = (float)r.v[v];
+        for (int v = 0; v < VEC; ++v) x[k][v] = (float)q.v[v];
       } else {
 #pragma unroll
-        for (int v = 0; v < VEC; ++v) x[k * VEC + v] = ck + v < c1 ? (float)z[ck + v] : -INFINITY;
+        for (int v = 0; v < VEC; ++v) x[k][v] = ck + v < c1 ? (float)z[ck + v] : -INFINITY;
       }
     }
-    t.add(x);
-    if (TOP) {
 #pragma unroll
-      for (int k = 0; k < U; ++k)
-#pragma unroll
-        for (int v = 0; v < VEC; ++v)
-          if (x[k * VEC + v] > best) best = x[k * VEC + v], best_c = c + (long)k * GT * VEC + v;
+    for (int k = 0; k < U; ++k) {
+      if (c + (long)k * GT * VEC >= c1) break;
+      t.add(x[k]);
     }
   }
+  const float best = t.m;  // of the thread's own classes
   t.join_wave();
   if (GT > 64) {
-    __shared__ float part[4][3];
+    __shared__ float part[GT / 64][3];
     const int w = tid >> 6;
     if ((tid & 63) == 0) part[w][0] = t.m, part[w][1] = t.s, part[w][2] = t.u;
     __syncthreads();
@@ -261,59 +411,66 @@ __global__ __launch_bounds__(256) void class_probs_forward_kernel(ProbArgs a) {
   const bool whole = a.nseg == 1;
   if (tid == 0) {
     if (whole) {
-      finish_row<E>(a, row, t);
+      finish_row(a, row, t, token);
     } else {
       float* p = a.part + (row * a.nseg + blockIdx.y) * 3;
       p[0] = t.m, p[1] = t.s, p[2] = t.u;
     }
   }
   if (TOP) {
-    __shared__ TopShared<GT> sh[256 / GT];
-    const long n = c1 - c0;
-    const int per = (int)((n + (long)GT * VEC - 1) / ((long)GT * VEC)) * VEC;
-    const u64 mine = c0 + (long)tid * VEC < c1 ? class_key(best, best_c) : 0;
+    __shared__ TopShared<GT> sh[kRows<GT>];
+    const unsigned mine = c0 + (long)tid * VEC < c1 ? value_bits(best) : 0;
     u64* list = whole ? nullptr : a.part_top + (row * a.nseg + blockIdx.y) * a.top;
-    if (!whole) {
-      // a segment may hold fewer classes than are wanted
-      for (long i = tid; i < a.top; i += GT)
-        if (i >= n) list[i] = 0;
-    }
-    select_top<GT>(
-        sh[grp], tid, a.top, mine, per,
-        [&](int th, int j) -> u64 {
-          const long c = c0 + ((long)(j / VEC) * GT + th) * VEC + j % VEC;
-          return c < c1 ? class_key((float)z[c], c) : 0;
-        },
-        [&](int r, u64 key) {
-          if (whole) emit_top(a, row, r, key, t);
-          else list[r] = key;
-        });
+    if (!whole && tid < a.top && tid >= c1 - c0) list[tid] = 0;  // a segment may hold fewer classes than are wanted
+    select_top<E, GT>(sh[grp], tid, a.top, mine, z, c0, c1, [&](int r, u64 key) {
+      if (whole) emit_top(a, row, r, key, t);
+      else list[r] = key;
+    });
   }
 }
 
-// One wave a row: joins the segments' statistics and merges their lists (one lane a segment).
+// One workgroup a row: the first wave joins the segments' statistics (a lane a segment); of the
+// segments' lists the keys that can be among the first `top` are ranked.
 template <typename E>
-__global__ __launch_bounds__(64) void class_probs_join_kernel(ProbArgs a) {
+__global__ __launch_bounds__(256) void class_probs_join_kernel(ProbArgs a) {
   const long row = blockIdx.x;
-  const int lane = threadIdx.x;
-  Sums t;
-  if (lane < a.nseg) {
-    const float* p = a.part + (row * a.nseg + lane) * 3;
-    t.m = p[0], t.s = p[1], t.u = p[2];
-  }
-  t.join_wave();
-  if (lane == 0) finish_row<E>(a, row, t);
-  const u64* list = a.part_top + (row * a.nseg + lane) * a.top;
-  int at = 0;
-  u64 head = lane < a.nseg && a.top > 0 ? list[0] : 0;
-  for (int r = 0; r < a.top; ++r) {
-    const u64 key = wave_max(head);
-    if (head == key) {
-      emit_top(a, row, r, key, t);
-      ++at;
-      head = at < a.top ? list[at] : 0;
+  const int tid = threadIdx.x;
+  __shared__ float whole[3];
+  __shared__ u64 tau;
+  __shared__ int count;
+  __shared__ u64 cand[kMaxSeg * kMaxTop];
+  const u64* list = a.part_top + row * a.nseg * a.top;
+  const int keys = a.nseg * a.top;
+  u64 key[kMaxSeg * kMaxTop / 256];
+#pragma unroll
+  for (int i = 0; i < kMaxSeg * kMaxTop / 256; ++i) key[i] = i * 256 + tid < keys ? list[i * 256 + tid] : 0;
+  if (tid < 64) {
+    const Token token(a, row, static_cast<const E*>(a.z) + row * a.ldz);
+    const bool has = tid < a.nseg && a.top > 0;
+    const u64 head = has ? list[(long)tid * a.top] : 0, tail = has ? list[(long)tid * a.top + a.top - 1] : 0;
+    Sums t;
+    if (tid < a.nseg) {
+      const float* p = a.part + (row * a.nseg + tid) * 3;
+      t.m = p[0], t.s = p[1], t.u = p[2];
+    }
+    t.join_wave();
+    // a.top keys reach the a.top-th of the segments' first keys, and the last key of any one segment
+    const u64 kth = a.top > 0 ? wave_kth(head, a.top) : 0, own = wave_max(tail);
+    if (tid == 0) {
+      finish_row(a, row, t, token);
+      whole[0] = t.m, whole[1] = t.s, whole[2] = t.u;
+      tau = kth > own ? kth : own ? own : 1, count = 0;
     }
   }
+  if (a.top == 0) return;
+  __syncthreads();
+  Sums t;
+  t.m = whole[0], t.s = whole[1], t.u = whole[2];
+#pragma unroll
+  for (int i = 0; i < kMaxSeg * kMaxTop / 256; ++i)
+    append(cand, &count, kMaxSeg * kMaxTop, key[i] >= tau, key[i]);
+  __syncthreads();
+  rank_out<256>(cand, count, tid, a.top, [&](int r, u64 k) { emit_top(a, row, r, k, t); });
 }
 
 // dz = -p (dlogp + dentropy (log p + H)), + dlogp at the token: one read, one write.
@@ -367,17 +524,22 @@ __global__ __launch_bounds__(256) void class_probs_backward_kernel(ProbArgs a, c
   }
 }
 
-constexpr long kWaveRow = 2048;  // up to this many classes one wave takes a row
 
-// Segments of a row: rows enough to fill the chip take one workgroup each; fewer rows are cut, a
-// segment no shorter than four vectors for each of its threads, at most one lane's worth in number.
+// A wave takes a row where rows are short, or many enough to fill the chip so (4096 rows of 50001
+// bf16 classes: 83 us, with a workgroup a row 90); else a workgroup does.
+bool wave_rows(long N, long V) { return V <= 2048 || N >= 4096; }
+
+// Segments of a row: where there are few long rows (below 16 rounds of a workgroup the second launch
+// costs more than it gives: 64 rows of 8192 fp32 classes 15.0 us cut, 11.4 whole) each is cut until
+// the chip is full, into pieces of two rounds at least (5 rows of 151001 fp16 classes with 20
+// alternatives: pieces of two rounds 15.6 us, of four 22.3, of eight 17.2).
 int row_segments(long N, long V, int vec, long* seg) {
   *seg = V;
-  if (V <= kWaveRow || N >= 512) return 1;
-  const long least = 256L * vec * 4;
+  const long round = 256L * vec;
+  if (wave_rows(N, V) || N >= 512 || V < 16 * round) return 1;
   long n = 512 / N;
-  if (n > (V + least - 1) / least) n = (V + least - 1) / least;
-  if (n > 64) n = 64;
+  if (n > (V + 2 * round - 1) / (2 * round)) n = (V + 2 * round - 1) / (2 * round);
+  if (n > kMaxSeg) n = kMaxSeg;
   long len = (V + n - 1) / n;
   len = (len + vec - 1) / vec * vec;
   *seg = len;
@@ -400,7 +562,7 @@ int check_rows(int dtype, long N, long V, long ldz) {
 
 template <typename E, bool TOP>
 int run_forward(ProbArgs a, hipStream_t s) {
-  if (a.V <= kWaveRow) {
+  if (wave_rows(a.N, a.V)) {
     class_probs_forward_kernel<E, 64, TOP><<<(unsigned)((a.N + 3) / 4), 256, 0, s>>>(a);
     AVC_LAUNCH_CHECK();
     return AVC_OK;
@@ -408,7 +570,7 @@ int run_forward(ProbArgs a, hipStream_t s) {
   class_probs_forward_kernel<E, 256, TOP><<<dim3((unsigned)a.N, a.nseg), 256, 0, s>>>(a);
   AVC_LAUNCH_CHECK();
   if (a.nseg > 1) {
-    class_probs_join_kernel<E><<<(unsigned)a.N, 64, 0, s>>>(a);
+    class_probs_join_kernel<E><<<(unsigned)a.N, 256, 0, s>>>(a);
     AVC_LAUNCH_CHECK();
   }
   return AVC_OK;

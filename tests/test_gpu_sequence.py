@@ -355,8 +355,14 @@ def test_log_probs_past_32_bit_offsets(cuda_device):
     z.normal_(generator=torch.Generator(device=cuda_device).manual_seed(2))
     tok = torch.full((N,), V - 1, device=cuda_device)
     a, b = ops.token_log_probs(z, tok, top=3), ops.token_log_probs(z[-600:].clone(), tok[-600:], top=3)
-    for x, y in zip(a, b):
-        assert torch.equal(x[-600:], y)
+    assert torch.equal(a[3][-600:], b[3])
+    # the two calls may lay rows over the chip differently: each is within the oracle's bound of the
+    # exact value, so they are within twice that of each other
+    Elp, EH, _ = so.log_probs_bounds(z[-20:].cpu(), tok[-20:].cpu())
+    half = [so.rounded(x[-20:].cpu().double(), torch.float32) for x in a[:3]]
+    _near(a[0][-20:], b[0][-20:].cpu().double(), 2 * (Elp[:, V - 1] + half[0]), "logp")
+    _near(a[1][-20:], b[1][-20:].cpu().double(), 2 * (EH + half[1]), "entropy")
+    _near(a[2][-20:], b[2][-20:].cpu().double(), 2 * (Elp.gather(1, a[3][-20:].cpu()) + half[2]), "top_logp")
 
 
 # ---- counter-based dropout --------------------------------------------------------------------------
