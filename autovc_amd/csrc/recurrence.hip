@@ -8,7 +8,7 @@
 // frame t hands to frame t - 1:  e_t = o_t dy_t + c_{t+1},  c_t = f_t e_t  (c behind the last frame
 // is the gradient of the final state), a stretch acts as c -> A c + B' with the same A, and
 //   dg_f = e_t (h_{t-1} - z) f (1 - f),  dg_c = e_t (1 - f)(1 - z^2),  dg_o = dy h_t o (1 - o).
-// h is formed again from states that the forward keeps every kStateStep frames.
+// h is formed again from states that the forward keeps every kChunk frames.
 //
 // Everything but the loaded and stored elements is fp32.  1 - f is never formed by subtraction.
 #include <algorithm>
@@ -19,11 +19,9 @@
 namespace avc {
 namespace {
 
-constexpr int kStateStep = 64;  // frames between the states that the forward keeps for the backward
-constexpr int kSF = 8;          // frames of a wave's stretch, all in registers (forward)
-constexpr int kSB = 8;          // ... (backward)
-constexpr int kW = 8;           // waves of a workgroup = stretches of its chunk
-static_assert(kStateStep % kSF == 0 && kSB * kW % kStateStep == 0, "a kept state is the state before a stretch");
+constexpr int kS = 8;            // frames of a wave's stretch, all in registers
+constexpr int kW = 8;            // waves of a workgroup = stretches of its chunk
+constexpr int kChunk = kS * kW;  // frames between the states that the forward keeps for the backward
 
 struct RecArgs {
   int T, B, H, dirs;
@@ -34,7 +32,7 @@ struct RecArgs {
   void* y;
   long ldy;
   float* hT;         // [D][B][H]
-  float* states;     // [ceil(T / kStateStep)][D][B][H]
+  float* states;     // [ceil(T / kChunk)][D][B][H]
   const void* dy;
   long lddy;
   const float* dhT;
@@ -46,26 +44,24 @@ struct RecArgs {
   int log_g, nct;    // lanes of a wave per row (log2), channel tiles per row
 };
 
-// Forget gate and its complement.  Below -80 (f < 2e-35) the exponential is held there, so that
-// neither it nor the reciprocal leaves the normal range; a NaN passes.
-__device__ __forceinline__ void forget_gate(float g, float& f, float& i) {
-  const float gc = g < -80.0f ? -80.0f : g;
-  const float e = __expf(-gc);
+// The forget gate as f = 1 / (1 + e), 1 - f = e f with e = exp(-g).  Below -80 (f < 2e-35) e is held
+// there, so that neither it nor f leaves the normal range; a NaN passes.
+__device__ __forceinline__ void forget_gate(float g, float& f, float& e) {
+  e = __expf(-__builtin_elementwise_maximum(g, -80.0f));
   f = __builtin_amdgcn_rcpf(1.0f + e);
-  i = e * f;
 }
-// tanh for 16-bit inputs: a shorter polynomial than gate_tanh's, error below 1e-6 relative
-__device__ __forceinline__ float tanh_short(float x) {
-  const float ax = fabsf(x), x2 = x * x;
-  float p = fmaf(x2, -0.0539682540f, 0.133333333f);
-  p = fmaf(p, x2, -0.333333333f);
-  const float small = fmaf(x * x2, p, x);
-  const float big = 1.0f - 2.0f * __builtin_amdgcn_rcpf(1.0f + __expf(2.0f * ax));
-  return ax < 0.15f ? small : copysignf(big, x);
-}
+// tanh x = 1 - 2 / (1 + exp 2x).  fp32 gates take gate_tanh, whose error is a few units relative
+// everywhere.  For 16-bit ones a cubic below 1/32 and the formula above it do: the formula is off by
+// 6 * 2^-24 absolutely at most (two instructions of 1 unit, a sum and a rounded argument, on a
+// reciprocal <= 1/2 taken twice), which at 1/32 is 192 * 2^-24 of the value -- below 2^-16, a
+// sixteenth of the half step that an fp16 gate itself was rounded by -- and the cubic by
+// 2/15 x^4 < 2^-22; 5 instructions less a gate.
 template <typename E>
 __device__ __forceinline__ float candidate(float x) {
-  return sizeof(E) == 4 ? gate_tanh(x) : tanh_short(x);
+  if (sizeof(E) == 4) return gate_tanh(x);
+  const float small = fmaf(x * x, x * -0.333333333f, x);
+  const float big = fmaf(-2.0f, __builtin_amdgcn_rcpf(1.0f + __expf(2.0f * x)), 1.0f);
+  return fabsf(x) < 0.03125f ? small : big;
 }
 
 // Where a lane works: VEC channels of one row b in one direction.  Rows narrower than a wave share
@@ -177,7 +173,6 @@ __device__ void join_segments(const RecArgs& a, int lo, int hi, const float* agg
 
 template <typename E, int VEC, bool RAGGED>
 __global__ __launch_bounds__(kW * 64, 4) void recurrence_forward_kernel(RecArgs a) {
-  constexpr int kS = kSF, kChunk = kS * kW;
   const Place<E, VEC> at(a);
   const int wave = at.wave, lane = at.lane;
   __shared__ float part[2][kW][2][64][VEC];
@@ -227,11 +222,10 @@ __global__ __launch_bounds__(kW * 64, 4) void recurrence_forward_kernel(RecArgs 
       for (int k = 0; k < kS; ++k)
 #pragma unroll
         for (int v = 0; v < VEC; ++v) {
-          float f, i;
-          forget_gate((float)rf[k].v[v], f, i);
-          const float z = candidate<E>((float)rc[k].v[v]);
+          float f, e;
+          forget_gate((float)rf[k].v[v], f, e);
           o[k][v] = gate_sigmoid((float)ro[k].v[v]);
-          loc[k][v] = Bv[v] = fmaf(f, Bv[v], i * z);
+          loc[k][v] = Bv[v] = f * fmaf(e, candidate<E>((float)rc[k].v[v]), Bv[v]);  // f h + (1 - f) z
           prod[k][v] = A[v] *= f;
         }
     }
@@ -250,7 +244,7 @@ __global__ __launch_bounds__(kW * 64, 4) void recurrence_forward_kernel(RecArgs 
       }
     }
     if (s0 >= a.T || !at.ok) continue;
-    if (a.states && s0 % kStateStep == 0) give<VEC>(a.states + (long)(s0 / kStateStep) * nstate + st0, soff, hin);
+    if (a.states && wave == 0) give<VEC>(a.states + (long)chunk * nstate + st0, soff, hin);
 #pragma unroll
     for (int k = 0; k < kS; ++k) {
       if (s0 + k < a.T) {
@@ -268,7 +262,6 @@ __global__ __launch_bounds__(kW * 64, 4) void recurrence_forward_kernel(RecArgs 
 
 template <typename E, int VEC, bool RAGGED>
 __global__ __launch_bounds__(kW * 64, 2) void recurrence_backward_kernel(RecArgs a) {
-  constexpr int kS = kSB, kChunk = kS * kW;
   const Place<E, VEC> at(a);
   const int wave = at.wave, lane = at.lane;
   __shared__ float part[2][kW][3][64][VEC];
@@ -290,7 +283,7 @@ __global__ __launch_bounds__(kW * 64, 2) void recurrence_backward_kernel(RecArgs
     const int s0 = chunk * kChunk + wave * kS;
     const Live live = live_of<RAGGED, kS>(a, s0, at.rev, at.len);
     if (live == kNone) return;
-    take_to<VEC>(hs, a.states + (long)(chunk * (kChunk / kStateStep)) * nstate + st0, soff);
+    take_to<VEC>(hs, a.states + (long)chunk * nstate + st0, soff);
     auto frame = [&](int k) {
       const int t = frame_of(a, s0 + k, at.rev);
       const E* p = g + t * gstep;
@@ -327,6 +320,7 @@ __global__ __launch_bounds__(kW * 64, 2) void recurrence_backward_kernel(RecArgs
 #pragma unroll
         for (int v = 0; v < VEC; ++v) {
           forget_gate((float)rf[k].v[v], f[k][v], i[k][v]);
+          i[k][v] *= f[k][v];
           z[k][v] = candidate<E>((float)rc[k].v[v]);
           o[k][v] = gate_sigmoid((float)ro[k].v[v]);
           d[k][v] = (float)ry[k].v[v];
@@ -408,8 +402,7 @@ __global__ __launch_bounds__(kW * 64, 2) void recurrence_backward_kernel(RecArgs
 // What one segment of time does to the state before it (BACK: to the gradient behind it): each
 // wave walks a run of stretches of its own, then the waves' runs are joined in order.
 template <typename E, int VEC, bool RAGGED, bool BACK>
-__global__ __launch_bounds__(kW * 64) void recurrence_segment_kernel(RecArgs a) {
-  constexpr int kS = BACK ? kSB : kSF;
+__global__ __launch_bounds__(kW * 64, 8) void recurrence_segment_kernel(RecArgs a) {
   const Place<E, VEC> at(a);
   const int wave = at.wave, lane = at.lane;
   __shared__ float part[kW][2][64][VEC];
@@ -418,16 +411,16 @@ __global__ __launch_bounds__(kW * 64) void recurrence_segment_kernel(RecArgs a) 
   const unsigned goff = at.off(a.ldg), dyoff = at.off(a.lddy), soff = at.off(a.H);
   const long gstep = (long)a.B * a.ldg, dystep = (long)a.B * a.lddy;
   const long st0 = at.state0(a), nstate = (long)(a.dirs == 3 ? 2 : 1) * a.B * a.H;
-  // seg_chunks chunks of kW stretches: seg_chunks stretches in a row for each wave
-  const int n = a.seg_chunks;
-  const int base = ((int)blockIdx.y * n * kW + wave * n) * kS;
+  const int steps = a.seg_chunks * kS;  // of a wave's run
+  const int base = ((int)blockIdx.y * kW + wave) * steps;
   float A[VEC], Bv[VEC];
 #pragma unroll
   for (int v = 0; v < VEC; ++v) A[v] = 1.0f, Bv[v] = 0.0f;
-  Vec<E, VEC> r0[kS], r1[kS], r2[kS];
-  auto load = [&](int q) {
-    const int s0 = base + (BACK ? n - 1 - q : q) * kS;
-    if (q >= n) return;
+  for (int q = 0; q < steps; q += kS) {
+    const int s0 = base + (BACK ? steps - kS - q : q);
+    const Live live = live_of<RAGGED, kS>(a, s0, at.rev, at.len);
+    if (live == kNone) continue;
+    Vec<E, VEC> r0[kS], r1[kS], r2[kS];
     auto frame = [&](int k) {
       const int t = frame_of(a, s0 + k, at.rev);
       const E* p = g + t * gstep;
@@ -439,43 +432,26 @@ __global__ __launch_bounds__(kW * 64) void recurrence_segment_kernel(RecArgs a) 
         r1[k] = take<VEC>(p + a.H, goff);
       }
     };
-    const Live live = live_of<RAGGED, kS>(a, s0, at.rev, at.len);
     if (live == kAll) {
 #pragma unroll
       for (int k = 0; k < kS; ++k) frame(k);
-    } else if (live == kPart) {
+    } else {
 #pragma unroll
       for (int k = 0; k < kS; ++k) {
         r0[k] = constant<E, VEC>(INFINITY), r1[k] = r2[k] = constant<E, VEC>(0.0f);
         if (is_live<RAGGED>(a, s0 + k, at.rev, at.len)) frame(k);
       }
     }
-  };
-  load(0);
-  for (int q = 0; q < n; ++q) {
-    const int s0 = base + (BACK ? n - 1 - q : q) * kS;
-    const Live live = live_of<RAGGED, kS>(a, s0, at.rev, at.len);
-    float f[kS][VEC], u[kS][VEC];
-    if (live != kNone) {
-#pragma unroll
-      for (int k = 0; k < kS; ++k)
-#pragma unroll
-        for (int v = 0; v < VEC; ++v) {
-          float i;
-          forget_gate((float)r0[k].v[v], f[k][v], i);
-          u[k][v] = BACK ? gate_sigmoid((float)r1[k].v[v]) * (float)r2[k].v[v]
-                         : i * candidate<E>((float)r1[k].v[v]);
-        }
-    }
-    load(q + 1);
-    if (live == kNone) continue;
 #pragma unroll
     for (int kk = 0; kk < kS; ++kk) {
       const int k = BACK ? kS - 1 - kk : kk;
 #pragma unroll
       for (int v = 0; v < VEC; ++v) {
-        Bv[v] = BACK ? f[k][v] * (u[k][v] + Bv[v]) : fmaf(f[k][v], Bv[v], u[k][v]);
-        A[v] *= f[k][v];
+        float f, e;
+        forget_gate((float)r0[k].v[v], f, e);
+        Bv[v] = f * (BACK ? fmaf(gate_sigmoid((float)r1[k].v[v]), (float)r2[k].v[v], Bv[v])
+                          : fmaf(e, candidate<E>((float)r1[k].v[v]), Bv[v]));
+        A[v] *= f;
       }
     }
   }
@@ -531,9 +507,9 @@ __global__ __launch_bounds__(256) void recurrence_step_kernel(int B, int H, cons
   }
 #pragma unroll
   for (int v = 0; v < VEC; ++v) {
-    float f, i;
-    forget_gate((float)rf.v[v], f, i);
-    hn[v] = fmaf(f, hv[v], i * candidate<E>((float)rc.v[v]));
+    float f, e;
+    forget_gate((float)rf.v[v], f, e);
+    hn[v] = f * fmaf(e, candidate<E>((float)rc.v[v]), hv[v]);
     out[v] = gate_sigmoid((float)ro.v[v]) * hn[v];
   }
   E* yo = y + (long)b * ldy + j;
@@ -548,7 +524,7 @@ __global__ __launch_bounds__(256) void recurrence_step_kernel(int B, int H, cons
 }
 
 // channels of a lane
-template <typename E, bool BACK>
+template <typename E>
 constexpr int wide() { return sizeof(E) == 4 ? 1 : 2; }
 
 // How a call is laid over the chip: lanes per row, row tiles, and segments of time.  With enough
@@ -557,10 +533,10 @@ constexpr int wide() { return sizeof(E) == 4 ? 1 : 2; }
 struct Layout {
   int log_g = 0, nct, nseg, seg_chunks;
   long tiles;
-  Layout(int T, int B, int H, int D, int vec, int chunk) {
+  Layout(int T, int B, int H, int D, int vec) {
     while (log_g < 6 && (vec << log_g) < H) ++log_g;
     nct = (H + (vec << log_g) - 1) / (vec << log_g);
-    const int rows = 64 >> log_g, chunks = (T + chunk - 1) / chunk;
+    const int rows = 64 >> log_g, chunks = (T + kChunk - 1) / kChunk;
     tiles = (long)nct * ((B + rows - 1) / rows);
     long n = tiles * D >= 256 ? 1 : 512 / (tiles * D);
     if (n > chunks) n = chunks;
@@ -570,16 +546,13 @@ struct Layout {
   size_t workspace(int B, int H, int D) const { return nseg > 1 ? (size_t)nseg * 2 * D * B * H * sizeof(float) : 0; }
 };
 
-template <typename E, bool BACK>
-Layout layout(int T, int B, int H, int D) {
-  const int vec = H >= wide<E, BACK>() ? wide<E, BACK>() : 1;
-  return Layout(T, B, H, D, vec, kW * (BACK ? kSB : kSF));
-}
+template <typename E>
+Layout layout(int T, int B, int H, int D) { return Layout(T, B, H, D, H >= wide<E>() ? wide<E>() : 1); }
 
 template <typename E, int VEC, bool BACK>
 int run_recurrence(RecArgs a, size_t ws_bytes, hipStream_t s) {
   const int D = a.dirs == 3 ? 2 : 1;
-  const Layout l = layout<E, BACK>(a.T, a.B, a.H, D);
+  const Layout l = layout<E>(a.T, a.B, a.H, D);
   a.log_g = l.log_g, a.nct = l.nct, a.nseg = l.nseg, a.seg_chunks = l.seg_chunks;
   const size_t need = l.workspace(a.B, a.H, D);
   AVC_CHECK_ARG(ws_bytes >= need && (need == 0 || a.agg), "workspace smaller than avc_gated_recurrence_workspace");
@@ -620,19 +593,15 @@ using namespace avc;
 
 extern "C" size_t avc_gated_recurrence_states(int T, int B, int H, int dirs) {
   if (T < 0 || B < 0 || H < 1 || dirs < 1 || dirs > 3) return 0;
-  return (size_t)(T / kStateStep + (T % kStateStep != 0)) * (dirs == 3 ? 2 : 1) * B * H;
+  return (size_t)(T / kChunk + (T % kChunk != 0)) * (dirs == 3 ? 2 : 1) * B * H;
 }
 
-// enough for either direction's call
 extern "C" size_t avc_gated_recurrence_workspace(int dtype, int T, int B, int H, int dirs) {
   if (!dtype_ok(dtype) || T < 1 || B < 1 || H < 1 || dirs < 1 || dirs > 3) return 0;
   const int D = dirs == 3 ? 2 : 1;
   size_t n = 0;
   with_dtype(dtype, [&](auto e) {
-    using E = decltype(e);
-    n = layout<E, false>(T, B, H, D).workspace(B, H, D);
-    const size_t m = layout<E, true>(T, B, H, D).workspace(B, H, D);
-    if (m > n) n = m;
+    n = layout<decltype(e)>(T, B, H, D).workspace(B, H, D);
     return AVC_OK;
   });
   return n;
@@ -652,7 +621,7 @@ extern "C" int avc_gated_recurrence_forward(int dtype, int T, int B, int H, int 
   a.y = y, a.ldy = ldy, a.hT = hT, a.states = states, a.agg = static_cast<float*>(workspace);
   return with_dtype(dtype, [&](auto e) {
     using E = decltype(e);
-    constexpr int V = wide<E, false>();
+    constexpr int V = wide<E>();
     return H >= V ? run_recurrence<E, V, false>(a, workspace_bytes, s)
                   : run_recurrence<E, 1, false>(a, workspace_bytes, s);
   });
@@ -674,7 +643,7 @@ extern "C" int avc_gated_recurrence_backward(int dtype, int T, int B, int H, int
   a.dh0 = dh0, a.agg = static_cast<float*>(workspace);
   return with_dtype(dtype, [&](auto e) {
     using E = decltype(e);
-    constexpr int V = wide<E, true>();
+    constexpr int V = wide<E>();
     return H >= V ? run_recurrence<E, V, true>(a, workspace_bytes, s)
                   : run_recurrence<E, 1, true>(a, workspace_bytes, s);
   });
