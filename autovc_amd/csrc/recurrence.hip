@@ -412,7 +412,9 @@ __global__ __launch_bounds__(kW * 64, 8) void recurrence_segment_kernel(RecArgs 
   const long gstep = (long)a.B * a.ldg, dystep = (long)a.B * a.lddy;
   const long st0 = at.state0(a), nstate = (long)(a.dirs == 3 ? 2 : 1) * a.B * a.H;
   const int steps = a.seg_chunks * kS;  // of a wave's run
-  const int base = ((int)blockIdx.y * kW + wave) * steps;
+  // (the last segment in the order of work acts on nothing)
+  const int seg = BACK ? blockIdx.y + 1 : blockIdx.y;
+  const int base = (seg * kW + wave) * steps;
   float A[VEC], Bv[VEC];
 #pragma unroll
   for (int v = 0; v < VEC; ++v) A[v] = 1.0f, Bv[v] = 0.0f;
@@ -459,7 +461,7 @@ __global__ __launch_bounds__(kW * 64, 8) void recurrence_segment_kernel(RecArgs 
   for (int v = 0; v < VEC; ++v) part[wave][0][lane][v] = A[v], part[wave][1][lane][v] = Bv[v];
   __syncthreads();
   if (wave == 0 && at.ok) {
-    float* p = a.agg + (long)blockIdx.y * 2 * nstate + st0;
+    float* p = a.agg + (long)seg * 2 * nstate + st0;
     float A2[VEC], B2[VEC];
 #pragma unroll
     for (int v = 0; v < VEC; ++v) {
@@ -523,13 +525,17 @@ __global__ __launch_bounds__(256) void recurrence_step_kernel(int B, int H, cons
   }
 }
 
-// channels of a lane
+// Channels of a lane: 4 bytes.  (8-byte lanes hold twice the registers: a training pass of
+// 128x256x512 took 60 + 106 us in fp32 instead of 53 + 101, 37 + 142 us in bf16 instead of 32 + 57.)
 template <typename E>
 constexpr int wide() { return sizeof(E) == 4 ? 1 : 2; }
 
-// How a call is laid over the chip: lanes per row, row tiles, and segments of time.  With enough
-// row tiles to fill the chip each workgroup walks its rows' whole time; with fewer, time is cut
-// into as many segments as bring the grid there.
+// How a call is laid over the chip: lanes per row, row tiles, and segments of time.  With row tiles
+// enough to fill the chip each workgroup walks its rows' whole time; with fewer, time is cut into as
+// many segments as bring the grid to two workgroups a CU, which costs a pass over most of the gates
+// for the segments' actions and a launch.  1024 frames in 128 tiles (bf16, ragged): cut in four
+// 42 us, whole 57; 60001 frames in 4 tiles: 128 segments 100 us, 64 111.  Up to 512 frames are not
+// cut: 400 frames in 180 tiles 36 us cut, 26 whole; 200 frames in 16 tiles 13 us either way.
 struct Layout {
   int log_g = 0, nct, nseg, seg_chunks;
   long tiles;
@@ -538,21 +544,19 @@ struct Layout {
     nct = (H + (vec << log_g) - 1) / (vec << log_g);
     const int rows = 64 >> log_g, chunks = (T + kChunk - 1) / kChunk;
     tiles = (long)nct * ((B + rows - 1) / rows);
-    long n = tiles * D >= 256 ? 1 : 512 / (tiles * D);
+    long n = tiles * D >= 256 || chunks <= 8 ? 1 : 512 / (tiles * D);
     if (n > chunks) n = chunks;
     seg_chunks = (int)((chunks + n - 1) / n);
     nseg = (chunks + seg_chunks - 1) / seg_chunks;
   }
   size_t workspace(int B, int H, int D) const { return nseg > 1 ? (size_t)nseg * 2 * D * B * H * sizeof(float) : 0; }
 };
-
 template <typename E>
 Layout layout(int T, int B, int H, int D) { return Layout(T, B, H, D, H >= wide<E>() ? wide<E>() : 1); }
 
 template <typename E, int VEC, bool BACK>
-int run_recurrence(RecArgs a, size_t ws_bytes, hipStream_t s) {
+int run_recurrence(RecArgs a, const Layout& l, size_t ws_bytes, hipStream_t s) {
   const int D = a.dirs == 3 ? 2 : 1;
-  const Layout l = layout<E>(a.T, a.B, a.H, D);
   a.log_g = l.log_g, a.nct = l.nct, a.nseg = l.nseg, a.seg_chunks = l.seg_chunks;
   const size_t need = l.workspace(a.B, a.H, D);
   AVC_CHECK_ARG(ws_bytes >= need && (need == 0 || a.agg), "workspace smaller than avc_gated_recurrence_workspace");
@@ -562,8 +566,9 @@ int run_recurrence(RecArgs a, size_t ws_bytes, hipStream_t s) {
   AVC_CHECK_ARG(widest < (1L << 29) >> (6 - l.log_g), "row stride too large");
   const dim3 grid((unsigned)l.tiles, a.nseg, D);
   if (a.nseg > 1) {
-    if (a.lengths) recurrence_segment_kernel<E, VEC, true, BACK><<<grid, kW * 64, 0, s>>>(a);
-    else recurrence_segment_kernel<E, VEC, false, BACK><<<grid, kW * 64, 0, s>>>(a);
+    const dim3 before((unsigned)l.tiles, a.nseg - 1, D);
+    if (a.lengths) recurrence_segment_kernel<E, VEC, true, BACK><<<before, kW * 64, 0, s>>>(a);
+    else recurrence_segment_kernel<E, VEC, false, BACK><<<before, kW * 64, 0, s>>>(a);
     AVC_LAUNCH_CHECK();
   }
   if constexpr (BACK) {
@@ -621,9 +626,9 @@ extern "C" int avc_gated_recurrence_forward(int dtype, int T, int B, int H, int 
   a.y = y, a.ldy = ldy, a.hT = hT, a.states = states, a.agg = static_cast<float*>(workspace);
   return with_dtype(dtype, [&](auto e) {
     using E = decltype(e);
-    constexpr int V = wide<E>();
-    return H >= V ? run_recurrence<E, V, false>(a, workspace_bytes, s)
-                  : run_recurrence<E, 1, false>(a, workspace_bytes, s);
+    const Layout l = layout<E>(T, B, H, D);
+    return H >= wide<E>() ? run_recurrence<E, wide<E>(), false>(a, l, workspace_bytes, s)
+                          : run_recurrence<E, 1, false>(a, l, workspace_bytes, s);
   });
 }
 
@@ -643,9 +648,9 @@ extern "C" int avc_gated_recurrence_backward(int dtype, int T, int B, int H, int
   a.dh0 = dh0, a.agg = static_cast<float*>(workspace);
   return with_dtype(dtype, [&](auto e) {
     using E = decltype(e);
-    constexpr int V = wide<E>();
-    return H >= V ? run_recurrence<E, V, true>(a, workspace_bytes, s)
-                  : run_recurrence<E, 1, true>(a, workspace_bytes, s);
+    const Layout l = layout<E>(T, B, H, D);
+    return H >= wide<E>() ? run_recurrence<E, wide<E>(), true>(a, l, workspace_bytes, s)
+                          : run_recurrence<E, 1, true>(a, l, workspace_bytes, s);
   });
 }
 
