@@ -1,8 +1,10 @@
 // Log-probabilities of given classes under rows of logits, with each row's entropy and its most
-// probable classes.  One pass over the logits keeps, for every thread,
-//   m = max z,   s = sum exp(z - m),   u = sum exp(z - m) (z - m),
-// moved to a new maximum m' by s' = s e^(m - m'), u' = (u + (m - m') s) e^(m - m').  Then
-//   log p_i = (z_i - m) - log s,   entropy = log s - u / s   (both terms >= 0: nothing cancels).
+// probable classes.  One pass over the logits keeps, for every thread, the maximum m so far and the
+// sums of e^(z - m) and e^(z - m) (z - m), moved to a new maximum m' by
+//   s' = s e^(m - m'),   u' = (u + (m - m') s) e^(m - m').
+// With the largest class kept apart (s = 1 + rest),
+//   log p_i = (z_i - m) - log1p(rest),   entropy = log1p(rest) - u / s   (both terms >= 0),
+// and the gradient needs log p_i + entropy = (z_i - m) - u / s: nothing cancels.
 // All statistics are fp32.
 //
 // The alternatives: every thread also keeps the largest class of its own slice of the row.  The k
@@ -10,7 +12,7 @@
 // (a class elsewhere has k classes above it), so only those slices are read again.
 // Classes are ordered by one 64-bit key, the value's bits made monotone above the complement of
 // the class number: larger values first, equal ones by the lower class, no two keys alike.
-#include <type_traits>
+#include <climits>
 
 #include "typed.h"
 
@@ -35,7 +37,7 @@ struct ProbArgs {
   long seg;  // classes of a segment
   float *logp, *entropy, *stats, *top_logp;
   long long* top_ids;
-  float* part;   // [N][nseg][3]: m, s, u of a segment
+  float* part;   // [N][nseg][4]: Sums of a segment
   u64* part_top; // [N][nseg][top]: its classes in order, 0 behind the last
 };
 
@@ -57,78 +59,102 @@ __device__ __forceinline__ long key_class(u64 k) { return 0xffffffffu - (unsigne
 // Reductions over a wave by data-parallel-primitive moves (a few cycles a step, where a shuffle
 // through the LDS crossbar takes some hundred): after four shifts the last lane of each row of 16
 // holds its row, two broadcasts join the rows in lane 63.  The order is the same in every run.
-template <int CTRL, int ROWS>
-__device__ __forceinline__ unsigned dpp_move(unsigned x, unsigned none) {
-  return (unsigned)__builtin_amdgcn_update_dpp((int)none, (int)x, CTRL, ROWS, 0xf, false);
-}
-template <typename T, typename Op, typename Step>
-__device__ __forceinline__ T dpp_reduce(T x, Op op, Step step) {
-  x = op(x, step(x, std::integral_constant<int, 0x111>{}, std::integral_constant<int, 0xf>{}));
-  x = op(x, step(x, std::integral_constant<int, 0x112>{}, std::integral_constant<int, 0xf>{}));
-  x = op(x, step(x, std::integral_constant<int, 0x114>{}, std::integral_constant<int, 0xf>{}));
-  x = op(x, step(x, std::integral_constant<int, 0x118>{}, std::integral_constant<int, 0xf>{}));
-  x = op(x, step(x, std::integral_constant<int, 0x142>{}, std::integral_constant<int, 0xa>{}));
-  x = op(x, step(x, std::integral_constant<int, 0x143>{}, std::integral_constant<int, 0xc>{}));
-  return x;
-}
-__device__ __forceinline__ float last_lane(float x) {
-  return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(x), 63));
-}
-__device__ __forceinline__ float wave_max(float x) {
-  return last_lane(dpp_reduce(
-      x, [](float p, float q) { return fmaxf(p, q); },
-      [](float p, auto ctrl, auto rows) {
-        return __uint_as_float(dpp_move<ctrl.value, rows.value>(__float_as_uint(p), 0xff800000u));
-      }));
+// `none`, which the op leaves any value with, stands in for lanes that a move does not reach.
+template <typename Op>
+__device__ __forceinline__ int dpp_reduce(int x, int none, Op op) {
+  x = op(x, __builtin_amdgcn_update_dpp(none, x, 0x111, 0xf, 0xf, false));
+  x = op(x, __builtin_amdgcn_update_dpp(none, x, 0x112, 0xf, 0xf, false));
+  x = op(x, __builtin_amdgcn_update_dpp(none, x, 0x114, 0xf, 0xf, false));
+  x = op(x, __builtin_amdgcn_update_dpp(none, x, 0x118, 0xf, 0xf, false));
+  x = op(x, __builtin_amdgcn_update_dpp(none, x, 0x142, 0xa, 0xf, false));
+  x = op(x, __builtin_amdgcn_update_dpp(none, x, 0x143, 0xc, 0xf, false));
+  return __builtin_amdgcn_readlane(x, 63);
 }
 __device__ __forceinline__ float wave_sum(float x) {
-  return last_lane(dpp_reduce(
-      x, [](float p, float q) { return p + q; },
-      [](float p, auto ctrl, auto rows) {
-        return __uint_as_float(dpp_move<ctrl.value, rows.value>(__float_as_uint(p), 0u));
-      }));
+  return __int_as_float(dpp_reduce(__float_as_int(x), 0, [](int p, int q) {
+    return __float_as_int(__int_as_float(p) + __int_as_float(q));
+  }));
+}
+// (as integers of the same order: a float maximum would first quiet what a move has brought)
+__device__ __forceinline__ float wave_max(float x) {
+  auto ordered = [](int b) { return b ^ ((b >> 31) & 0x7fffffff); };
+  return __int_as_float(ordered(dpp_reduce(ordered(__float_as_int(x)), INT_MIN, [](int p, int q) { return max(p, q); })));
 }
 __device__ __forceinline__ u64 wave_max(u64 x) {
-  x = dpp_reduce(
-      x, [](u64 p, u64 q) { return q > p ? q : p; },
-      [](u64 p, auto ctrl, auto rows) {
-        const unsigned lo = dpp_move<ctrl.value, rows.value>((unsigned)p, 0u);
-        return (u64)dpp_move<ctrl.value, rows.value>((unsigned)(p >> 32), 0u) << 32 | lo;
-      });
-  return (u64)(unsigned)__builtin_amdgcn_readlane((unsigned)(x >> 32), 63) << 32 |
-         (unsigned)__builtin_amdgcn_readlane((unsigned)x, 63);
+  auto most = [](unsigned p) {
+    return (unsigned)dpp_reduce((int)p, 0, [](int a, int b) { return (int)max((unsigned)a, (unsigned)b); });
+  };
+  const unsigned hi = most((unsigned)(x >> 32));
+  return (u64)hi << 32 | most((unsigned)(x >> 32) == hi ? (unsigned)x : 0u);
 }
 
+// What a part of a row adds up to, about the largest logit m seen: s = sum e^(z - m) over the classes
+// below m, c = the classes at m, u = sum e^(z - m) (z - m).  The largest class is kept out of s
+// because the rest is what a confident row's entropy and log-probability are made of: in a sum
+// that begins with its 1 they would lose what lies below 2^-24.  A wave's lanes share m, so that
+// classes at or above it are a branch that a wave seldom takes.
 struct Sums {
-  float m = -INFINITY, s = 0.0f, u = 0.0f;
-  // to the maximum `to` >= m (-inf: nothing seen yet)
-  __device__ void move(float to) {
-    const float d = fmaxf(m - (to == -INFINITY ? 0.0f : to), kFar);
-    const float e = __expf(d);
-    u = fmaf(d, s, u) * e;
-    s *= e;
+  float m = -INFINITY, s = 0.0f, c = 0.0f, u = 0.0f;
+  // to a maximum `to` > m (or a part that has seen nothing)
+  __device__ __forceinline__ void move(float to) {
+    const float d = fmaxf(m - to, kFar);
+    const float e = __expf(d), all = s + c;
+    u = fmaf(d, all, u) * e;
+    s = all * e;
+    c = 0.0f;
     m = to;
   }
+  // the wave's next N classes a lane; `own`, the largest of the lane's
   template <int N>
-  __device__ void add(const float (&z)[N]) {
-    float top = m;
+  __device__ __forceinline__ void add(const float (&z)[N], float& own) {
+    float top = z[0];
 #pragma unroll
-    for (int k = 0; k < N; ++k) top = fmaxf(top, z[k]);
-    move(top);
-    const float mm = top == -INFINITY ? 0.0f : top;
+    for (int k = 1; k < N; ++k) top = fmaxf(top, z[k]);
+    own = fmaxf(own, top);
+    if (!__any(top >= m)) {
+#pragma unroll
+      for (int k = 0; k < N; ++k) {
+        const float d = __builtin_elementwise_maximum(z[k] - m, kFar);  // (a NaN passes)
+        const float e = __expf(d);
+        s += e;
+        u = fmaf(e, d, u);
+      }
+      return;
+    }
+    const float most = wave_max(top);
+    if (most > m) move(most);
+    const float mm = m == -INFINITY ? 0.0f : m;
+    float below = 0.0f;
 #pragma unroll
     for (int k = 0; k < N; ++k) {
-      const float d = z[k] - mm;
+      const float d = __builtin_elementwise_maximum(z[k] - mm, kFar);
       const float e = __expf(d);
-      s += e;
-      u = fmaf(e, fmaxf(d, kFar), u);
+      const float less = __builtin_amdgcn_fmed3f(d * -0x1p126f, 0.0f, 1.0f);  // 0 at m, else 1
+      s = fmaf(e, less, s);
+      below += less;
+      u = fmaf(e, d, u);
     }
+    c += (float)N - below;
   }
-  __device__ void join_wave() {
-    move(wave_max(m));
+  __device__ __forceinline__ void join_wave() {
     s = wave_sum(s);
     u = wave_sum(u);
+    // mostly one lane holds the one class at m
+    c = __any(c > 1.0f) ? wave_sum(c) : (float)__popcll(__ballot(c == 1.0f));
   }
+};
+
+// A row's result: its largest logit, the others' sum against it, and the mean of m - z under p
+struct RowStats {
+  float m, rest, mean;
+  bool none;  // nothing left in the row (a NaN row has a NaN sum)
+  __device__ explicit RowStats(const Sums& t) : m(t.m) {
+    none = t.m == -INFINITY && t.s == 0.0f;
+    rest = none ? 0.0f : t.s + (t.c - 1.0f);
+    mean = none ? 0.0f : -t.u / (1.0f + rest);
+  }
+  __device__ explicit RowStats(const float* p) : m(p[0]), rest(p[1]), mean(p[2]) { none = m == -INFINITY && rest == 0.0f; }
+  __device__ float log_sum() const { return log1pf(rest); }
 };
 
 // barrier among the GT threads that share a row (one wave's LDS operations stay in order)
@@ -314,24 +340,19 @@ struct Token {
 };
 
 // one thread: the row's statistics and its token's log-probability
-__device__ __forceinline__ void finish_row(const ProbArgs& a, long row, const Sums& t, const Token& k) {
-  // nothing left in the row (a NaN row has a NaN sum)
-  const bool none = t.m == -INFINITY && t.s == 0.0f;
-  const float logs = none ? 0.0f : logf(t.s);
-  const float H = none ? 0.0f : logs - t.u / t.s;
-  a.entropy[row] = H;
-  if (a.stats) a.stats[row * 3] = t.m, a.stats[row * 3 + 1] = t.s, a.stats[row * 3 + 2] = H;
+__device__ __forceinline__ void finish_row(const ProbArgs& a, long row, const RowStats& t, const Token& k) {
+  const float logs = t.log_sum();
+  a.entropy[row] = logs + t.mean;
+  if (a.stats) a.stats[row * 3] = t.m, a.stats[row * 3 + 1] = t.rest, a.stats[row * 3 + 2] = t.mean;
   float lp;
   if (k.tok == a.ignore) lp = 0.0f;
   else if (k.tok < 0 || k.tok >= a.V) lp = NAN;
-  else if (none) lp = -INFINITY;
+  else if (t.none) lp = -INFINITY;
   else lp = (k.z - t.m) - logs;
   a.logp[row] = lp;
 }
-__device__ __forceinline__ void emit_top(const ProbArgs& a, long row, int r, u64 key, const Sums& t) {
-  const float z = key_value(key);
-  const bool none = t.m == -INFINITY && t.s == 0.0f;
-  a.top_logp[row * a.top + r] = none ? -INFINITY : (z - t.m) - logf(t.s);
+__device__ __forceinline__ void emit_top(const ProbArgs& a, long row, int r, u64 key, const RowStats& t) {
+  a.top_logp[row * a.top + r] = t.none ? -INFINITY : (key_value(key) - t.m) - t.log_sum();
   a.top_ids[row * a.top + r] = key_class(key);
 }
 
@@ -351,6 +372,7 @@ __global__ __launch_bounds__(GT * kRows<GT>) void class_probs_forward_kernel(Pro
   const long c0 = (long)blockIdx.y * a.seg, c1 = c0 + a.seg < a.V ? c0 + a.seg : a.V;
   const Token token(a, row, z);
   Sums t;
+  float own = -INFINITY;  // the largest of the thread's classes
   Vec<E, VEC> r[U];
   long c = c0;
   auto load = [&](long from) {
@@ -365,7 +387,7 @@ __global__ __launch_bounds__(GT * kRows<GT>) void class_probs_forward_kernel(Pro
 #pragma unroll
       for (int v = 0; v < VEC; ++v) x[k][v] = (float)r[k].v[v];
     if (c + 2 * kRound <= c1) load(c + kRound);
-    t.add(reinterpret_cast<const float(&)[U * VEC]>(x));
+    t.add(reinterpret_cast<const float(&)[U * VEC]>(x), own);
   }
   if (c < c1) {  // less than a round is left, its last vector perhaps cut
     float x[U][VEC];
@@ -384,15 +406,14 @@ __global__ __launch_bounds__(GT * kRows<GT>) void class_probs_forward_kernel(Pro
 #pragma unroll
     for (int k = 0; k < U; ++k) {
       if (c + (long)k * GT * VEC >= c1) break;
-      t.add(x[k]);
+      t.add(x[k], own);
     }
   }
-  const float best = t.m;  // of the thread's own classes
   t.join_wave();
   if (GT > 64) {
-    __shared__ float part[GT / 64][3];
+    __shared__ float part[GT / 64][4];
     const int w = tid >> 6;
-    if ((tid & 63) == 0) part[w][0] = t.m, part[w][1] = t.s, part[w][2] = t.u;
+    if ((tid & 63) == 0) part[w][0] = t.m, part[w][1] = t.s, part[w][2] = t.c, part[w][3] = t.u;
     __syncthreads();
     float m = -INFINITY;
 #pragma unroll
@@ -402,28 +423,29 @@ __global__ __launch_bounds__(GT * kRows<GT>) void class_probs_forward_kernel(Pro
 #pragma unroll
     for (int i = 0; i < GT / 64; ++i) {
       Sums p;
-      p.m = part[i][0], p.s = part[i][1], p.u = part[i][2];
-      p.move(m);
-      all.s += p.s, all.u += p.u;
+      p.m = part[i][0], p.s = part[i][1], p.c = part[i][2], p.u = part[i][3];
+      if (m > p.m) p.move(m);
+      all.s += p.s, all.c += p.c, all.u += p.u;
     }
     t = all;
   }
   const bool whole = a.nseg == 1;
   if (tid == 0) {
     if (whole) {
-      finish_row(a, row, t, token);
+      finish_row(a, row, RowStats(t), token);
     } else {
-      float* p = a.part + (row * a.nseg + blockIdx.y) * 3;
-      p[0] = t.m, p[1] = t.s, p[2] = t.u;
+      float* p = a.part + (row * a.nseg + blockIdx.y) * 4;
+      p[0] = t.m, p[1] = t.s, p[2] = t.c, p[3] = t.u;
     }
   }
   if (TOP) {
     __shared__ TopShared<GT> sh[kRows<GT>];
-    const unsigned mine = c0 + (long)tid * VEC < c1 ? value_bits(best) : 0;
+    const unsigned mine = c0 + (long)tid * VEC < c1 ? value_bits(own) : 0;
     u64* list = whole ? nullptr : a.part_top + (row * a.nseg + blockIdx.y) * a.top;
     if (!whole && tid < a.top && tid >= c1 - c0) list[tid] = 0;  // a segment may hold fewer classes than are wanted
+    const RowStats st(t);
     select_top<E, GT>(sh[grp], tid, a.top, mine, z, c0, c1, [&](int r, u64 key) {
-      if (whole) emit_top(a, row, r, key, t);
+      if (whole) emit_top(a, row, r, key, st);
       else list[r] = key;
     });
   }
@@ -450,22 +472,24 @@ __global__ __launch_bounds__(256) void class_probs_join_kernel(ProbArgs a) {
     const u64 head = has ? list[(long)tid * a.top] : 0, tail = has ? list[(long)tid * a.top + a.top - 1] : 0;
     Sums t;
     if (tid < a.nseg) {
-      const float* p = a.part + (row * a.nseg + tid) * 3;
-      t.m = p[0], t.s = p[1], t.u = p[2];
+      const float* p = a.part + (row * a.nseg + tid) * 4;
+      t.m = p[0], t.s = p[1], t.c = p[2], t.u = p[3];
     }
+    const float most = wave_max(t.m);
+    if (most > t.m) t.move(most);
     t.join_wave();
     // a.top keys reach the a.top-th of the segments' first keys, and the last key of any one segment
     const u64 kth = a.top > 0 ? wave_kth(head, a.top) : 0, own = wave_max(tail);
     if (tid == 0) {
-      finish_row(a, row, t, token);
-      whole[0] = t.m, whole[1] = t.s, whole[2] = t.u;
+      const RowStats st(t);
+      finish_row(a, row, st, token);
+      whole[0] = st.m, whole[1] = st.rest, whole[2] = st.mean;
       tau = kth > own ? kth : own ? own : 1, count = 0;
     }
   }
   if (a.top == 0) return;
   __syncthreads();
-  Sums t;
-  t.m = whole[0], t.s = whole[1], t.u = whole[2];
+  const RowStats t(whole);
 #pragma unroll
   for (int i = 0; i < kMaxSeg * kMaxTop / 256; ++i)
     append(cand, &count, kMaxSeg * kMaxTop, key[i] >= tau, key[i]);
@@ -473,7 +497,8 @@ __global__ __launch_bounds__(256) void class_probs_join_kernel(ProbArgs a) {
   rank_out<256>(cand, count, tid, a.top, [&](int r, u64 k) { emit_top(a, row, r, k, t); });
 }
 
-// dz = -p (dlogp + dentropy (log p + H)), + dlogp at the token: one read, one write.
+// dz = dlogp (onehot - p) - dentropy p ((z - m) + mean): one read, one write.  1 - p of the largest
+// class is rest / (1 + rest).
 template <typename E>
 __global__ __launch_bounds__(256) void class_probs_backward_kernel(ProbArgs a, const float* dlogp,
                                                                    const float* dentropy, void* dz, long lddz,
@@ -485,13 +510,12 @@ __global__ __launch_bounds__(256) void class_probs_backward_kernel(ProbArgs a, c
   const long c0 = (long)(item % tiles) * (64 * VEC * U) + (threadIdx.x & 63) * VEC;
   const E* z = static_cast<const E*>(a.z) + row * a.ldz;
   E* d = static_cast<E*>(dz) + row * lddz;
-  const float m = a.stats[row * 3], s = a.stats[row * 3 + 1], H = a.stats[row * 3 + 2];
-  const bool none = m == -INFINITY && s == 0.0f;
+  const RowStats t(a.stats + row * 3);
   const long long tok = a.tokens[row];
   const bool bad = tok != a.ignore && (tok < 0 || tok >= a.V);
   const float gl = !dlogp || tok == a.ignore ? 0.0f : bad ? NAN : dlogp[row];
   const float ge = dentropy ? dentropy[row] : 0.0f;
-  const float inv = 1.0f / s, off = H - logf(s);
+  const float inv = 1.0f / (1.0f + t.rest);
 #pragma unroll
   for (int k = 0; k < U; ++k) {
     const long c = c0 + (long)k * 64 * VEC;
@@ -508,11 +532,12 @@ __global__ __launch_bounds__(256) void class_probs_backward_kernel(ProbArgs a, c
     }
 #pragma unroll
     for (int v = 0; v < VEC; ++v) {
-      const float e = x[v] - m;
+      const float e = x[v] - t.m;
       const float p = __expf(e) * inv;
-      float g = -p * fmaf(ge, fmaxf(e, kFar) + off, gl);
-      if (c + v == tok) g += gl;
-      x[v] = !none ? g : gl != gl ? gl : 0.0f;
+      const float through = ge * (fmaxf(e, kFar) + t.mean);
+      float g = -p * (through + gl);
+      if (c + v == tok) g = fmaf(gl, e == 0.0f ? t.rest * inv : 1.0f - p, -p * through);
+      x[v] = !t.none ? g : gl != gl ? gl : 0.0f;
     }
     if (full) {
       vstore<E, VEC>(d + c, x);

@@ -442,7 +442,8 @@ int avc_gated_recurrence_step(int dtype, int B, int H, const void* gates, long l
  *   logits   [N] rows of V, stride ldz; -inf rules a class out
  *   tokens   [N]: the class of each row.  ignore_index gives log-probability 0 and no gradient through it;
  *            any other value outside 0 .. V-1 gives NaN, and NaN through dlogp in the row's gradient
- *   logp, entropy [N]; stats [N][3] kept for the backward (row maximum m, sum of exp(z - m), entropy)
+ *   logp, entropy [N]; stats [N][3] kept for the backward (row maximum m, sum of exp(z - m)
+ *            less its largest term, mean of m - z)
  *   top_logp, top_ids [N][top], top in 0 .. min(32, V): log-probabilities and classes, most probable
  *            first, equal ones by the lower class; a NaN logit ranks as -inf
  * A row in which every class is ruled out has log-probability -inf (top_logp too), entropy 0 and gradient 0.

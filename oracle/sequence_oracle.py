@@ -102,9 +102,18 @@ def recurrence_bounds(gates, T, B, h0=None, lengths=None, dirs=1, dy=None, dhT=N
 
 # ---- log-probabilities of given classes -----------------------------------------------------------
 def log_softmax(z):
-    """From the differences to the maximum: at logits of -3e38 even float64 holds no z - lse."""
+    """From the differences to the maximum (at logits of -3e38 even float64 holds no z - lse), and with
+    the largest class kept out of the sum (a confident row's rest is below its 1's last bit)."""
     d = z - z.max()
-    return d - torch.logsumexp(d, 0)
+    others = torch.ones_like(d, dtype=torch.bool)
+    others[d.argmax()] = False
+    return d - torch.log1p(torch.exp(d[others]).sum())
+
+
+def entropy_of(lp):
+    """Of log-probabilities along the last dimension (0 log 0 = 0)."""
+    p = torch.exp(lp)
+    return -torch.where(p > 0, p * lp, torch.zeros_like(p)).sum(-1)
 
 
 def log_probs(logits, tokens, top=0, ignore_index=-100):
@@ -115,7 +124,7 @@ def log_probs(logits, tokens, top=0, ignore_index=-100):
     for r in range(N):
         if not bool((z[r] == -math.inf).all()):
             lp[r] = log_softmax(z[r])
-    entropy = torch.special.entr(torch.exp(lp)).sum(1)
+    entropy = entropy_of(lp)
     logp = torch.zeros(N, dtype=torch.float64)
     for r, t in enumerate(tokens.tolist()):
         if t != ignore_index:
@@ -138,10 +147,10 @@ def log_probs_grad(logits, tokens, dlogp, dentropy, ignore_index=-100):
             continue
         lp = log_softmax(z[r])
         p = torch.exp(lp)
-        plp = -torch.special.entr(p)
-        d[r] = -gl * p - float(dentropy[r]) * (plp - p * plp.sum())
+        plus = float(dentropy[r]) * p * (torch.where(p > 0, lp, torch.zeros_like(lp)) + entropy_of(lp))
+        d[r] = -gl * p - plus
         if 0 <= t < V:
-            d[r, t] += gl
+            d[r, t] = -gl * torch.expm1(lp[t]) - plus[t]  # gl (1 - p), not from 1 - p
     return d
 
 

@@ -328,6 +328,34 @@ def test_log_probs_nan_inf_and_bad_tokens(cuda_device):
         assert ops.token_log_probs(z[:1].to(cuda_device), torch.tensor([-1], device=cuda_device), ignore_index=-1)[0].item() == 0
 
 
+@pytest.mark.parametrize("V", [2, 40, 3000, 40000])
+def test_log_probs_of_confident_rows(cuda_device, V):
+    """Rows whose largest class leaves the others 1e-2 .. 1e-14: entropy, log-probability and gradient
+    keep their relative precision (in a sum that begins with the largest class's 1 they would not)."""
+    gen = torch.Generator().manual_seed(V)
+    z = torch.randn(16, V, generator=gen)
+    top = torch.randint(0, V, (16,), generator=gen)
+    z[torch.arange(16), top] = z.max() + torch.linspace(2.0, 22.0, 16) + math.log(V)
+    logp, H, _, _ = so.log_probs(z, top)
+    leaf = z.to(cuda_device).requires_grad_(True)
+    got = ops.token_log_probs(leaf, top.to(cuda_device))
+    # every term of these sums of like signs is off by (|d| + 3) U and each of at most 300 additions by
+    # one: all of it relative to the result, |d| <= 45 here
+    rel = 350 * so.U
+    _near(got[0], logp, rel * logp.abs(), "logp")
+    _near(got[1], H, rel * H, "entropy")
+    ones = torch.ones(16)
+    for gl, ge in ((ones, 0 * ones), (0 * ones, ones)):
+        d = torch.autograd.grad((got[0], got[1]), leaf, (gl.to(cuda_device), ge.to(cuda_device)), retain_graph=True)[0].cpu().double()
+        ref = so.log_probs_grad(z, top, gl, ge)
+        hot = torch.zeros(16, V, dtype=torch.bool)
+        hot[torch.arange(16), top] = True
+        # dlogp: 1 - p at the token, -p elsewhere; dentropy: p (|d| - mean) with |d| far above mean
+        # elsewhere, p mean at the token
+        assert ((d - ref).abs() <= 2 * rel * ref.abs())[hot if gl[0] else ~hot].all()
+        assert ((d - ref).abs() <= 2 * rel * ref.abs())[hot].all()
+
+
 def test_log_probs_shapes_and_gradients_of_one_output(cuda_device):
     gen = torch.Generator().manual_seed(4)
     z, tok = torch.randn(2, 3, 20, generator=gen), torch.randint(0, 20, (2, 3), generator=gen)
