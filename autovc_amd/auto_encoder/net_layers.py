@@ -1,4 +1,5 @@
-"""Parameter-holding layers with the reference's names and init (net_layers.py:3-49).
+"""Parameter-holding layers with the reference's names and init (net_layers.py:3-49), and the gated
+linear recurrence layer.
 
 ConvNorm / LinearNorm keep `.conv` / `.linear_layer` (torch Conv1d / Linear) so state_dict keys,
 shapes and Xavier-uniform init match the reference exactly; their arithmetic never runs through
@@ -8,6 +9,8 @@ import math
 
 import torch
 import torch.nn as nn
+
+from .. import ops
 
 
 class LinearNorm(nn.Module):
@@ -65,3 +68,42 @@ class LSTMParams(nn.Module):
 
     def flatten_parameters(self):  # encoder.py:74 calls this on nn.LSTM; nothing to do here
         return None
+
+
+class GatedRecurrence(nn.Module):
+    """A gated linear recurrence layer over time-major frames [T*B][C]: one projection to the gates
+    (f, c, o of each direction, as rows [D][3][H] of `weight_ih`), then ops.gated_recurrence.  It
+    stands where an nn.LSTM layer stands (decoder.py:37, encoder.py:51) when time is long: its cost
+    does not grow with the number of steps in sequence.
+
+    Initialised as LSTMParams (U(+-1/sqrt(H))), with the forget gates' bias raised by `forget_bias`
+    so that a fresh layer remembers."""
+
+    def __init__(self, input_size, hidden_size, bidirectional=False, reverse=False, forget_bias=1.0):
+        super().__init__()
+        if bidirectional and reverse:
+            raise ValueError("a layer is bidirectional or reverse, not both")
+        if input_size % 4 or hidden_size % 4:
+            raise ValueError("the projection's products take widths that are multiples of 4")
+        self.input_size, self.hidden_size = input_size, hidden_size
+        self.dirs = 3 if bidirectional else 2 if reverse else 1
+        D = 2 if bidirectional else 1
+        self.weight_ih = nn.Parameter(torch.empty(D * 3 * hidden_size, input_size))
+        self.bias_ih = nn.Parameter(torch.empty(D * 3 * hidden_size))
+        stdv = 1.0 / math.sqrt(hidden_size)
+        nn.init.uniform_(self.weight_ih, -stdv, stdv)
+        nn.init.uniform_(self.bias_ih, -stdv, stdv)
+        with torch.no_grad():
+            self.bias_ih.view(D, 3, hidden_size)[:, 0].add_(forget_bias)
+
+    def forward(self, x, T, B, h0=None, lengths=None):
+        """x [T*B][input_size] -> (y [T*B][D*H], last states [D][B][H]); see ops.gated_recurrence."""
+        return ops.gated_recurrence(ops.Linear.apply(x, self.weight_ih, self.bias_ih), T, B, h0, lengths, self.dirs)
+
+    @torch.no_grad()
+    def step(self, x, state):
+        """One frame of a forward layer, state [B][H] updated in place: x [B][input_size] -> y [B][H]."""
+        if self.dirs != 1:
+            raise ValueError("only a forward layer can be stepped")
+        gates = ops.Linear.apply(x, self.weight_ih, self.bias_ih)
+        return ops.gated_recurrence_step(gates, state, out_state=state)[0]

@@ -640,7 +640,7 @@ __global__ __launch_bounds__(64) void lstm32_fwd_kernel(int T, int B, long ldgx,
     const long row = (long)t * B + b;
     float a0, a1, fg, og;
     if constexpr (FAST) {
-      // packed FMAs (v_pk_fma_f32: two k per instruction), two chains of 8 per gate row
+      // FMAs in pairs of k, two chains of 8 pairs per gate row
       typedef float f2 __attribute__((ext_vector_type(2)));
       f2 q0[2] = {f2{0.f, 0.f}, f2{0.f, 0.f}}, q1[2] = {f2{0.f, 0.f}, f2{0.f, 0.f}};
 #pragma unroll
@@ -883,8 +883,8 @@ int launch_lstm32(int nblk, int T, int B, long ldgx, long ldy, const L32Dir& d0,
 // saved gates, c_t, c_{t-1}) come from a register ring whose next group is requested before a
 // group's steps (loop unrolled by PF: static slots; clamped, so no join waits on them), and the dG broadcast through LDS needs
 // no barrier: one wave's LDS operations complete in issue order (see lstm32_fwd_kernel).
-// FAST (round 4, avc_lstm32_tune(1), the default): the 64-term dot product as two packed-FMA
-// chains (v_pk_fma_f32, 16 instructions deep each, instead of one 64-deep scalar chain), and
+// FAST (avc_lstm32_tune(1), the default): the 64-term dot product as two chains of FMA pairs
+// (each 16 pairs deep, instead of one 64-deep scalar chain), and
 // tanh(c_t) in the forward FAST kernel's own form, so the derivative uses the very tanh(c) value
 // the forward multiplied by o_t (libm tanhf was also the longest piece of the step's chain).
 template <int PF, bool FAST = false>

@@ -25,7 +25,7 @@ import numpy as np
 import torch
 import torch.nn as nn
 
-from .. import _lib
+from .. import _lib, ops
 from ..hparams import WaveRNNParams
 
 _M = WaveRNNParams["model"]
@@ -191,6 +191,17 @@ class WaveRNN(nn.Module):
         with torch.no_grad():
             _, logits, _ = self._run(mels, False, 0, 0, 0, x_teacher=x)
         return logits
+
+    def log_probs(self, x, mels, classes, top=0):
+        """How probable the RAW model finds given sample classes: forward(x, mels), then
+        ops.token_log_probs of `classes` (1, L) -> (log-probabilities (1, L), entropies (1, L), and the
+        `top` most probable classes with their log-probabilities (1, L, top)).  A class of -100 is
+        left out (0).  Its mean is the RAW loss's negative (model.py:310-317 samples these classes)."""
+        if self.mode != "RAW":
+            raise ValueError("log_probs scores RAW classes; a MOL model's outputs are mixture parameters")
+        logits = self.forward(x, mels)
+        classes = torch.as_tensor(classes, device=logits.device)
+        return ops.token_log_probs(logits, classes, top=top)
 
     def generate(self, melspectrogram, batched=_G["batched"], target=_G["target"], overlap=_G["overlap"],
                  mu_law=_G["mu_law"]):
