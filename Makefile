@@ -11,8 +11,19 @@ SRC      := $(wildcard autovc_amd/csrc/*.hip)
 HDR      := $(wildcard autovc_amd/csrc/*.h) include/autovc_hip.h include/autovc_hip_debug.h
 OBJ      := $(patsubst autovc_amd/csrc/%.hip,build/%.o,$(SRC))
 LIB      := autovc_amd/libautovc_hip.so
+# the sequence-model operators as torch functions (a Python module over the C ABI, no GPU code)
+EXT      := autovc_amd/_sequence.so
+PY       ?= python3
+TORCH    := $(shell $(PY) -c "import importlib.util as u, os; print(os.path.dirname(u.find_spec('torch').origin))")
+PYINC    := $(shell $(PY) -c "import sysconfig; print(sysconfig.get_paths()['include'])")
 
-all: $(LIB)
+all: $(LIB) $(EXT)
+
+$(EXT): autovc_amd/csrc_torch/sequence.cpp include/autovc_hip.h Makefile
+	$(CXX) -O2 -std=c++17 -fPIC -shared -Wall -Wno-sign-compare -D__HIP_PLATFORM_AMD__=1 -DUSE_ROCM=1 \
+	  -DTORCH_EXTENSION_NAME=_sequence -isystem $(TORCH)/include -isystem $(TORCH)/include/torch/csrc/api/include \
+	  -isystem /opt/rocm/include -isystem $(PYINC) $< -o $@ \
+	  -L$(TORCH)/lib -lc10 -lc10_hip -ltorch_cpu -ltorch -ltorch_python -ldl
 
 # per-file machine-scheduler strategy (round 6, same-box A/B in DESIGN §9p): the persistent
 # recurrences schedule for instruction-level parallelism
@@ -31,7 +42,7 @@ check-abi: $(LIB)
 	python3 -c "import re,ctypes;lib=ctypes.CDLL('$(LIB)');n=[re.findall(r'^\w[\w\s\*]*?\b(avc_\w+)\(',open(f).read(),re.M) for f in ('include/autovc_hip.h','include/autovc_hip_debug.h')];[getattr(lib,x) for v in n for x in v];print(len(n[0]),'product +',len(n[1]),'debug symbols ok')"
 
 clean:
-	rm -rf build $(LIB)
+	rm -rf build $(LIB) $(EXT)
 
 .PHONY: all clean check-abi
 

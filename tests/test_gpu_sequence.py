@@ -662,3 +662,18 @@ def test_refusals(cuda_device):
     for bad in (dict(rng=r.float()), dict(residual=torch.zeros(8, 12, dtype=torch.float16, device=dev))):
         with pytest.raises(TypeError):
             ops.dropout(g, **({"p": 0.5, "rng": r} | bad))
+
+
+def test_gradients_are_differentiable_once(cuda_device):
+    """create_graph is allowed; using the graph of a gradient is an error, not a silent zero."""
+    dev = cuda_device
+    g = torch.randn(12, 9, device=dev, requires_grad=True)
+    w = torch.randn(12, 3, device=dev, requires_grad=True)
+    calls = [lambda: ops.gated_recurrence(g, 6, 2)[0] * w, lambda: ops.dropout(g, 0.5, _rng(dev))[:, :3] * w,
+             lambda: ops.token_log_probs(g, torch.zeros(12, dtype=torch.int64, device=dev))[0][:, None] * w]
+    for call in calls:
+        d = torch.autograd.grad(call().sum(), g)[0]
+        d2 = torch.autograd.grad(call().sum(), g, create_graph=True)[0]
+        assert torch.equal(d, d2.detach()) and d2.requires_grad
+        with pytest.raises(RuntimeError, match="differentiate twice"):
+            torch.autograd.grad(d2.sum(), w)
