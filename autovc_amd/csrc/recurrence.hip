@@ -8,7 +8,7 @@
 // frame t hands to frame t - 1:  e_t = o_t dy_t + c_{t+1},  c_t = f_t e_t  (c behind the last frame
 // is the gradient of the final state), a stretch acts as c -> A c + B' with the same A, and
 //   dg_f = e_t (h_{t-1} - z) f (1 - f),  dg_c = e_t (1 - f)(1 - z^2),  dg_o = dy h_t o (1 - o).
-// h is formed again from states that the forward keeps every kChunk frames.
+// h is formed again from states that the forward keeps every kState frames.
 //
 // Everything but the loaded and stored elements is fp32.  1 - f is never formed by subtraction.
 #include <algorithm>
@@ -19,9 +19,14 @@
 namespace avc {
 namespace {
 
-constexpr int kS = 8;            // frames of a wave's stretch, all in registers
-constexpr int kW = 8;            // waves of a workgroup = stretches of its chunk
-constexpr int kChunk = kS * kW;  // frames between the states that the forward keeps for the backward
+constexpr int kW = 8;        // waves of a workgroup = stretches of its chunk
+constexpr int kState = 32;   // frames between the states that the forward keeps for the backward
+// Frames of a wave's stretch, all in registers.  The backward of two-channel lanes takes 4, which
+// leaves room for a third workgroup a CU (128x256x512 bf16: 48 us, with 8 frames 56).
+template <int VEC, bool BACK>
+constexpr int stretch() { return BACK && VEC > 1 ? 4 : 8; }
+template <int VEC, bool BACK>
+constexpr int chunk_of() { return stretch<VEC, BACK>() * kW; }
 
 struct RecArgs {
   int T, B, H, dirs;
@@ -32,7 +37,7 @@ struct RecArgs {
   void* y;
   long ldy;
   float* hT;         // [D][B][H]
-  float* states;     // [ceil(T / kChunk)][D][B][H]
+  float* states;     // [ceil(T / kState)][D][B][H]
   const void* dy;
   long lddy;
   const float* dhT;
@@ -173,6 +178,7 @@ __device__ void join_segments(const RecArgs& a, int lo, int hi, const float* agg
 
 template <typename E, int VEC, bool RAGGED>
 __global__ __launch_bounds__(kW * 64, 4) void recurrence_forward_kernel(RecArgs a) {
+  constexpr int kS = stretch<VEC, false>(), kChunk = kS * kW;
   const Place<E, VEC> at(a);
   const int wave = at.wave, lane = at.lane;
   __shared__ float part[2][kW][2][64][VEC];
@@ -244,7 +250,7 @@ __global__ __launch_bounds__(kW * 64, 4) void recurrence_forward_kernel(RecArgs 
       }
     }
     if (s0 >= a.T || !at.ok) continue;
-    if (a.states && wave == 0) give<VEC>(a.states + (long)chunk * nstate + st0, soff, hin);
+    if (a.states && s0 % kState == 0) give<VEC>(a.states + (long)(s0 / kState) * nstate + st0, soff, hin);
 #pragma unroll
     for (int k = 0; k < kS; ++k) {
       if (s0 + k < a.T) {
@@ -262,6 +268,8 @@ __global__ __launch_bounds__(kW * 64, 4) void recurrence_forward_kernel(RecArgs 
 
 template <typename E, int VEC, bool RAGGED>
 __global__ __launch_bounds__(kW * 64, 2) void recurrence_backward_kernel(RecArgs a) {
+  constexpr int kS = stretch<VEC, true>(), kChunk = kS * kW;
+  static_assert(kChunk % kState == 0, "a chunk begins at a kept state");
   const Place<E, VEC> at(a);
   const int wave = at.wave, lane = at.lane;
   __shared__ float part[2][kW][3][64][VEC];
@@ -283,7 +291,7 @@ __global__ __launch_bounds__(kW * 64, 2) void recurrence_backward_kernel(RecArgs
     const int s0 = chunk * kChunk + wave * kS;
     const Live live = live_of<RAGGED, kS>(a, s0, at.rev, at.len);
     if (live == kNone) return;
-    take_to<VEC>(hs, a.states + (long)chunk * nstate + st0, soff);
+    take_to<VEC>(hs, a.states + (long)(chunk * (kChunk / kState)) * nstate + st0, soff);
     auto frame = [&](int k) {
       const int t = frame_of(a, s0 + k, at.rev);
       const E* p = g + t * gstep;
@@ -403,6 +411,7 @@ __global__ __launch_bounds__(kW * 64, 2) void recurrence_backward_kernel(RecArgs
 // wave walks a run of stretches of its own, then the waves' runs are joined in order.
 template <typename E, int VEC, bool RAGGED, bool BACK>
 __global__ __launch_bounds__(kW * 64, 8) void recurrence_segment_kernel(RecArgs a) {
+  constexpr int kS = stretch<VEC, BACK>();
   const Place<E, VEC> at(a);
   const int wave = at.wave, lane = at.lane;
   __shared__ float part[kW][2][64][VEC];
@@ -539,24 +548,27 @@ constexpr int wide() { return sizeof(E) == 4 ? 1 : 2; }
 struct Layout {
   int log_g = 0, nct, nseg, seg_chunks;
   long tiles;
-  Layout(int T, int B, int H, int D, int vec) {
+  Layout(int T, int B, int H, int D, int vec, int chunk) {
     while (log_g < 6 && (vec << log_g) < H) ++log_g;
     nct = (H + (vec << log_g) - 1) / (vec << log_g);
-    const int rows = 64 >> log_g, chunks = (T + kChunk - 1) / kChunk;
+    const int rows = 64 >> log_g, chunks = (T + chunk - 1) / chunk;
     tiles = (long)nct * ((B + rows - 1) / rows);
-    long n = tiles * D >= 256 || chunks <= 8 ? 1 : 512 / (tiles * D);
+    long n = tiles * D >= 256 || T <= 512 ? 1 : 512 / (tiles * D);
     if (n > chunks) n = chunks;
     seg_chunks = (int)((chunks + n - 1) / n);
     nseg = (chunks + seg_chunks - 1) / seg_chunks;
   }
   size_t workspace(int B, int H, int D) const { return nseg > 1 ? (size_t)nseg * 2 * D * B * H * sizeof(float) : 0; }
 };
-template <typename E>
-Layout layout(int T, int B, int H, int D) { return Layout(T, B, H, D, H >= wide<E>() ? wide<E>() : 1); }
+template <typename E, bool BACK>
+Layout layout(int T, int B, int H, int D) {
+  return H >= wide<E>() ? Layout(T, B, H, D, wide<E>(), chunk_of<wide<E>(), BACK>()) : Layout(T, B, H, D, 1, chunk_of<1, BACK>());
+}
 
 template <typename E, int VEC, bool BACK>
-int run_recurrence(RecArgs a, const Layout& l, size_t ws_bytes, hipStream_t s) {
+int run_recurrence(RecArgs a, size_t ws_bytes, hipStream_t s) {
   const int D = a.dirs == 3 ? 2 : 1;
+  const Layout l = layout<E, BACK>(a.T, a.B, a.H, D);
   a.log_g = l.log_g, a.nct = l.nct, a.nseg = l.nseg, a.seg_chunks = l.seg_chunks;
   const size_t need = l.workspace(a.B, a.H, D);
   AVC_CHECK_ARG(ws_bytes >= need && (need == 0 || a.agg), "workspace smaller than avc_gated_recurrence_workspace");
@@ -598,7 +610,7 @@ using namespace avc;
 
 extern "C" size_t avc_gated_recurrence_states(int T, int B, int H, int dirs) {
   if (T < 0 || B < 0 || H < 1 || dirs < 1 || dirs > 3) return 0;
-  return (size_t)(T / kChunk + (T % kChunk != 0)) * (dirs == 3 ? 2 : 1) * B * H;
+  return (size_t)(T / kState + (T % kState != 0)) * (dirs == 3 ? 2 : 1) * B * H;
 }
 
 extern "C" size_t avc_gated_recurrence_workspace(int dtype, int T, int B, int H, int dirs) {
@@ -606,7 +618,8 @@ extern "C" size_t avc_gated_recurrence_workspace(int dtype, int T, int B, int H,
   const int D = dirs == 3 ? 2 : 1;
   size_t n = 0;
   with_dtype(dtype, [&](auto e) {
-    n = layout<decltype(e)>(T, B, H, D).workspace(B, H, D);
+    using E = decltype(e);  // enough for either direction's call
+    n = std::max(layout<E, false>(T, B, H, D).workspace(B, H, D), layout<E, true>(T, B, H, D).workspace(B, H, D));
     return AVC_OK;
   });
   return n;
@@ -626,9 +639,8 @@ extern "C" int avc_gated_recurrence_forward(int dtype, int T, int B, int H, int 
   a.y = y, a.ldy = ldy, a.hT = hT, a.states = states, a.agg = static_cast<float*>(workspace);
   return with_dtype(dtype, [&](auto e) {
     using E = decltype(e);
-    const Layout l = layout<E>(T, B, H, D);
-    return H >= wide<E>() ? run_recurrence<E, wide<E>(), false>(a, l, workspace_bytes, s)
-                          : run_recurrence<E, 1, false>(a, l, workspace_bytes, s);
+    return H >= wide<E>() ? run_recurrence<E, wide<E>(), false>(a, workspace_bytes, s)
+                          : run_recurrence<E, 1, false>(a, workspace_bytes, s);
   });
 }
 
@@ -648,9 +660,8 @@ extern "C" int avc_gated_recurrence_backward(int dtype, int T, int B, int H, int
   a.dh0 = dh0, a.agg = static_cast<float*>(workspace);
   return with_dtype(dtype, [&](auto e) {
     using E = decltype(e);
-    const Layout l = layout<E>(T, B, H, D);
-    return H >= wide<E>() ? run_recurrence<E, wide<E>(), true>(a, l, workspace_bytes, s)
-                          : run_recurrence<E, 1, true>(a, l, workspace_bytes, s);
+    return H >= wide<E>() ? run_recurrence<E, wide<E>(), true>(a, workspace_bytes, s)
+                          : run_recurrence<E, 1, true>(a, workspace_bytes, s);
   });
 }
 
