@@ -251,13 +251,16 @@ __device__ void select_top(TopShared<GT>& sh, int tid, int k, unsigned mine, con
       }
     }
   };
-  slices([&](bool in, float x, long c) {
-    append(sh.cand, &sh.count, kCap, in && value_bits(x) >= tau, class_key(x, c));
-  });
-  row_sync<GT>();
-  if (sh.count <= kCap) {
-    rank_out<GT>(sh.cand, sh.count, tid, k, emit);
-    return;
+  // (tau stands at -inf where fewer than k classes are left: all the others are equal then)
+  if (tau > value_bits(-INFINITY)) {
+    slices([&](bool in, float x, long c) {
+      append(sh.cand, &sh.count, kCap, in && value_bits(x) >= tau, class_key(x, c));
+    });
+    row_sync<GT>();
+    if (sh.count <= kCap) {
+      rank_out<GT>(sh.cand, sh.count, tid, k, emit);
+      return;
+    }
   }
   // More candidates than fit: classes equal to tau, as where fewer than k are not ruled out.  Those
   // above it go first, then the lowest of the equal ones, looked for from the row's beginning.

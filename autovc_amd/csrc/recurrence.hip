@@ -410,8 +410,8 @@ __global__ __launch_bounds__(kW * 64, 2) void recurrence_backward_kernel(RecArgs
 // What one segment of time does to the state before it (BACK: to the gradient behind it): each
 // wave walks a run of stretches of its own, then the waves' runs are joined in order.
 template <typename E, int VEC, bool RAGGED, bool BACK>
-__global__ __launch_bounds__(kW * 64, 8) void recurrence_segment_kernel(RecArgs a) {
-  constexpr int kS = stretch<VEC, BACK>();
+__global__ __launch_bounds__(kW * 64, 6) void recurrence_segment_kernel(RecArgs a) {
+  constexpr int kS = 16;  // frames in flight (with 4 the ragged backward's took 17 us, with 16 it takes 15)
   const Place<E, VEC> at(a);
   const int wave = at.wave, lane = at.lane;
   __shared__ float part[kW][2][64][VEC];
@@ -420,7 +420,7 @@ __global__ __launch_bounds__(kW * 64, 8) void recurrence_segment_kernel(RecArgs 
   const unsigned goff = at.off(a.ldg), dyoff = at.off(a.lddy), soff = at.off(a.H);
   const long gstep = (long)a.B * a.ldg, dystep = (long)a.B * a.lddy;
   const long st0 = at.state0(a), nstate = (long)(a.dirs == 3 ? 2 : 1) * a.B * a.H;
-  const int steps = a.seg_chunks * kS;  // of a wave's run
+  const int steps = a.seg_chunks * stretch<VEC, BACK>();  // of a wave's run
   // (the last segment in the order of work acts on nothing)
   const int seg = BACK ? blockIdx.y + 1 : blockIdx.y;
   const int base = (seg * kW + wave) * steps;
@@ -428,7 +428,7 @@ __global__ __launch_bounds__(kW * 64, 8) void recurrence_segment_kernel(RecArgs 
 #pragma unroll
   for (int v = 0; v < VEC; ++v) A[v] = 1.0f, Bv[v] = 0.0f;
   for (int q = 0; q < steps; q += kS) {
-    const int s0 = base + (BACK ? steps - kS - q : q);
+    const int s0 = base + (BACK ? max(steps - q - kS, 0) : q), n = min(kS, steps - q);
     const Live live = live_of<RAGGED, kS>(a, s0, at.rev, at.len);
     if (live == kNone) continue;
     Vec<E, VEC> r0[kS], r1[kS], r2[kS];
@@ -443,14 +443,14 @@ __global__ __launch_bounds__(kW * 64, 8) void recurrence_segment_kernel(RecArgs 
         r1[k] = take<VEC>(p + a.H, goff);
       }
     };
-    if (live == kAll) {
+    if (live == kAll && n == kS) {
 #pragma unroll
       for (int k = 0; k < kS; ++k) frame(k);
     } else {
 #pragma unroll
       for (int k = 0; k < kS; ++k) {
         r0[k] = constant<E, VEC>(INFINITY), r1[k] = r2[k] = constant<E, VEC>(0.0f);
-        if (is_live<RAGGED>(a, s0 + k, at.rev, at.len)) frame(k);
+        if (k < n && is_live<RAGGED>(a, s0 + k, at.rev, at.len)) frame(k);
       }
     }
 #pragma unroll
