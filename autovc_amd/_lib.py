@@ -241,7 +241,7 @@ def ptr(t) -> int | None:
     return t.data_ptr()
 
 
-# element types of the sequence-model operators (AVC_DTYPE_*)
+# element types of the sequence-model entry points (AVC_DTYPE_*)
 DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 
 TIMING_CLASSES = {"gemm": 0, "lstm_step_fwd": 1, "lstm_step_bwd": 2, "lstm32": 3, "dft64": 4, "lstm2_persist": 5,

@@ -257,6 +257,7 @@ std::tuple<Tensor, Tensor> gated_recurrence_step(const Tensor& gates, const Tens
   if (out_state) {
     out = *out_state;
     check_type(out, "out_state", gates, at::kFloat, at::kFloat);
+    TORCH_CHECK(!wants_grad(out), "out_state is written in place, so it cannot require a gradient");
     TORCH_CHECK_VALUE(fits(out) && out.is_contiguous(), "out_state must be a contiguous [", B, ", ", H, "]");
     TORCH_CHECK_VALUE(!overlap(out, state) || (out.data_ptr() == state.data_ptr() && state.is_contiguous()),
                       "out_state overlaps state without being it");
@@ -389,14 +390,16 @@ struct Dropout : torch::autograd::Function<Dropout> {
     ctx->saved_data["needs"] = (x.requires_grad() ? 1 : 0) | (residual && residual->requires_grad() ? 2 : 0);
     return drop(x, residual.value_or(Tensor()), p, rng, layer);
   }
-  static variable_list backward(AutogradContext* ctx, variable_list d) { return once(d, grads(ctx, d)); }
-  static variable_list grads(AutogradContext* ctx, const variable_list& d) {
+  static variable_list backward(AutogradContext* ctx, variable_list d) {
+    const long needs = ctx->saved_data["needs"].toInt();
+    // (the residual's gradient is the incoming one itself, which keeps its own history)
+    return {needs & 1 ? once(d, {grad_x(ctx, d[0])})[0] : Tensor(), needs & 2 ? d[0] : Tensor(), Tensor(), Tensor(), Tensor()};
+  }
+  static Tensor grad_x(AutogradContext* ctx, const Tensor& dy) {
     // (rng is saved, so that changing it in place before the backward is an error and not another mask)
     const Tensor rng = ctx->get_saved_variables()[0];
-    const long needs = ctx->saved_data["needs"].toInt();
     const at::NoGradGuard plain;
-    Tensor dx = needs & 1 ? drop(d[0], Tensor(), ctx->saved_data["p"].toDouble(), rng, ctx->saved_data["layer"].toInt()) : Tensor();
-    return {dx, needs & 2 ? d[0] : Tensor(), Tensor(), Tensor(), Tensor()};
+    return drop(dy, Tensor(), ctx->saved_data["p"].toDouble(), rng, ctx->saved_data["layer"].toInt());
   }
 };
 

@@ -5,7 +5,9 @@ checks, allocation and autograd: csrc_torch/sequence.cpp).
 They take fp32, bf16 and fp16 tensors; statistics, sums and recurrent states are fp32.  Rows may be
 column slices of a wider buffer (any row stride); other layouts are made contiguous.  Every call
 runs on the current stream of its tensors' device and allocates what it needs through torch, so it
-may be captured into a graph and used from several streams.  Gradients are differentiable once.
+may be captured into a graph and used from several streams.  (A backward pass is captured only while no
+graph that was built outside the capture from the same leaves is alive, as torch asks for any of
+its own.)  Gradients are differentiable once.
 Public names are re-exported by `autovc_amd.ops`.
 """
 from __future__ import annotations

@@ -677,3 +677,28 @@ def test_gradients_are_differentiable_once(cuda_device):
         assert torch.equal(d, d2.detach()) and d2.requires_grad
         with pytest.raises(RuntimeError, match="differentiate twice"):
             torch.autograd.grad(d2.sum(), w)
+
+
+def test_dropout_hands_the_residuals_gradient_through(cuda_device):
+    """The incoming gradient is the residual's own: it stays what it was (a leaf here), and a graph
+    through it goes on."""
+    dev = cuda_device
+    x, res, w = (torch.randn(4, 6, device=dev, requires_grad=True) for _ in range(3))
+    y = ops.dropout(x, 0.5, _rng(dev), residual=res)
+    dx, dres = torch.autograd.grad(y, (x, res), w, create_graph=True)
+    assert w.is_leaf and w.grad_fn is None
+    assert torch.equal(dres, w)
+    dw, = torch.autograd.grad((dres * dres).sum(), w)
+    assert torch.equal(dw, 2 * w)
+    with pytest.raises(RuntimeError, match="differentiate twice"):
+        torch.autograd.grad(dx.sum(), w)
+
+
+def test_step_refuses_an_out_state_that_requires_a_gradient(cuda_device):
+    dev = cuda_device
+    s = torch.zeros(2, 4, device=dev, requires_grad=True)
+    with pytest.raises(RuntimeError, match="out_state"):
+        ops.gated_recurrence_step(torch.zeros(2, 12, device=dev), torch.zeros(2, 4, device=dev), out_state=s)
+    with torch.no_grad():
+        ops.gated_recurrence_step(torch.zeros(2, 12, device=dev), torch.ones(2, 4, device=dev), out_state=s)
+    assert torch.equal(s.detach(), torch.full((2, 4), 0.5, device=dev))
