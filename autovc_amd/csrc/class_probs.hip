@@ -13,6 +13,7 @@
 // Classes are ordered by one 64-bit key, the value's bits made monotone above the complement of
 // the class number: larger values first, equal ones by the lower class, no two keys alike.
 #include <climits>
+#include <utility>
 
 #include "typed.h"
 
@@ -272,7 +273,7 @@ __device__ void select_top(TopShared<GT>& sh, int tid, int k, unsigned mine, con
   });
   row_sync<GT>();
   const int above = sh.count;
-  if (above <= kCap - k) {
+  if (above <= kCap) {
     int have = above;
     for (long base = c0; base < c1 && have < k; base += (long)GT * VEC) {
       const long c = base + (long)tid * VEC;
@@ -361,6 +362,8 @@ __device__ __forceinline__ void emit_top(const ProbArgs& a, long row, int r, u64
 
 // GT threads a row segment: a wave, four of them a workgroup, or a workgroup of 256 (blockIdx.y is
 // the segment).  A thread reads U vectors at a time and asks for the next U before it adds the first.
+// Bound by the one read of the logits: 4096 rows of 50001 bf16 classes 83 us, 4.9 TB/s.  Few rows are
+// bound by the chain of load, reduction and store: one of 512 fp32 classes with 5 alternatives 5 us.
 template <int GT>
 constexpr int kRows = GT == 64 ? 4 : 1;  // rows of a workgroup
 
@@ -454,8 +457,192 @@ __global__ __launch_bounds__(GT * kRows<GT>) void class_probs_forward_kernel(Pro
   }
 }
 
+// Many rows of at most kShort classes: a wave takes four of them, 16 lanes each, whole in registers,
+// which spares three quarters of what a row costs beside its classes (reductions, logarithms) -- with
+// a wave a row that is what bounds it.  35200 rows of 512 fp32 classes 14.6 us (4.9 TB/s, the rate of a
+// large copy), with a wave a row 19.9; with 5 alternatives 26 and 38; 60000 rows of 100 fp32 classes with
+// 5 alternatives 18 and 57.  (Up to 20 alternatives it is never slower there; 32 of 512 classes 47 and 45.)
+constexpr int kShort = 512;
+constexpr int kShortCand = 64;  // candidates of a row that are ranked at once
+
+// the value J lanes round the lane's 16
+template <int J>
+__device__ __forceinline__ float turned(float x) {
+  return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), 0x120 + J, 0xf, 0xf, true));
+}
+// a sum or maximum over 16 lanes, the same bits in each of them
+template <typename Op>
+__device__ __forceinline__ float reduce16(float x, Op op) {
+  x = op(x, turned<8>(x));
+  x = op(x, turned<4>(x));
+  x = op(x, turned<2>(x));
+  return op(x, turned<1>(x));
+}
+__device__ __forceinline__ float max16(float x) {
+  return reduce16(x, [](float p, float q) { return fmaxf(p, q); });
+}
+// how many of the other 15 lanes' values are at least v
+template <int... J>
+__device__ __forceinline__ int at_least(float x, float v, std::integer_sequence<int, J...>) {
+  return (0 + ... + (int)(turned<J + 1>(x) >= v));
+}
+// A value that k of a row's classes are known to reach, the highest that the lanes' R largest tell
+// (-inf where they do not).
+template <int R, int M>
+__device__ __forceinline__ float reached(const float (&x)[M], int k) {
+  float best[R];
+#pragma unroll
+  for (int r = 0; r < R; ++r) best[r] = -INFINITY;
+#pragma unroll
+  for (int i = 0; i < M; ++i) {
+    float v = R == 1 ? x[i] : fmaxf(x[i], -INFINITY);  // (a NaN ranks as -inf)
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      const float less = fminf(best[r], v);
+      best[r] = fmaxf(best[r], v);
+      v = less;
+    }
+  }
+  float tau = -INFINITY;
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    int n = r + 1;
+#pragma unroll
+    for (int q = 0; q < R; ++q)
+      n += at_least(best[q], best[r], std::make_integer_sequence<int, 15>()) + (q > r && best[q] >= best[r]);
+    if (n >= k) tau = fmaxf(tau, best[r]);
+  }
+  return max16(tau);
+}
+
+// select_top for a row that 16 lanes hold: x[i] is class (i / VEC) 16 VEC + l VEC + i % VEC of V.
+// `live`: the row exists.
+template <typename E, int M, typename Emit>
+__device__ void select_short(u64* cand, int k, const float (&x)[M], const E* z, int V, bool live, Emit emit) {
+  constexpr int VEC = width<E>();
+  const int lane = threadIdx.x & 63, l = lane & 15, shift = lane & 48;
+  auto class_of = [&](int i) { return i / VEC * 16 * VEC + l * VEC + i % VEC; };
+  // the lanes of the row for which `in` holds: those before this one, and all
+  auto count = [&](bool in, int& before) {
+    const unsigned m = (unsigned)(__ballot(in) >> shift) & 0xffffu;
+    before = __popc(m & ((1u << l) - 1));
+    return __popc(m);
+  };
+  // of as many of the lanes' largest as let about k, and seldom more than the list holds, reach it
+  const float tau = k <= 8 ? reached<1>(x, k) : k <= 16 ? reached<2>(x, k) : reached<4>(x, k);
+  int n = 0;
+  auto gather = [&](auto wanted) {
+    n = 0;
+#pragma unroll
+    for (int i = 0; i < M; ++i) {
+      const bool in = wanted(x[i]);
+      if (!__any(in)) continue;
+      int before;
+      const int all = count(in, before);
+      if (in && n + before < kShortCand) cand[n + before] = class_key(x[i], class_of(i));
+      n += all;
+    }
+    row_sync<64>();
+  };
+  auto rank = [&](int n) {
+    for (int i = l; i < n; i += 16) {
+      const u64 key = cand[i];
+      int r = 0;
+      for (int j = 0; j < n; ++j) r += cand[j] > key;
+      if (r < k && live) emit(r, key);
+    }
+    row_sync<64>();
+  };
+  const bool some = tau > -INFINITY;
+  if (__any(some)) gather([&](float v) { return some && v >= tau; });
+  const bool few = some && n <= kShortCand;
+  if (__any(few)) rank(few ? n : 0);
+  if (!__any(!few)) return;
+  // as in select_top: those above tau, then the first of those at tau
+  gather([&](float v) { return !few && v > tau; });
+  const bool ties = !few && n <= kShortCand;
+  int have = ties ? n : k;
+  for (int base = 0; __any(have < k && base < V); base += 16) {
+    const int c = base + l;
+    const float v = c < V ? (float)z[c] : 0.0f;
+    int before;
+    const bool in = have < k && c < V && value_bits(v) == value_bits(tau);
+    const int all = count(in, before);
+    if (in && have + before < k) cand[have + before] = class_key(v, c);
+    have += all;
+  }
+  row_sync<64>();
+  rank(ties ? (n > k ? n : k) : 0);
+  if (!__any(!few && !ties)) return;
+  u64 under = !few && !ties ? ~0ull : 0;
+  for (int r = 0; r < k; ++r) {
+    u64 most = 0;
+#pragma unroll 1
+    for (int c = l; c < V; c += 16) {
+      const u64 key = class_key((float)z[c], c);
+      if (key < under && key > most) most = key;
+    }
+    for (int by = 8; by; by >>= 1) {
+      const u64 other = __shfl_xor(most, by);
+      most = other > most ? other : most;
+    }
+    under = most;
+    if (l == 0 && live && most != 0) emit(r, most);
+  }
+}
+
+template <typename E, int NV, bool TOP>
+__global__ __launch_bounds__(256) void class_probs_short_kernel(ProbArgs a) {
+  constexpr int VEC = width<E>(), kAcross = 16 * VEC;
+  const int l = threadIdx.x & 15;
+  const long at = (long)blockIdx.x * 16 + (threadIdx.x >> 4), row = at < a.N ? at : a.N - 1;
+  const E* z = static_cast<const E*>(a.z) + row * a.ldz;
+  const int V = (int)a.V;
+  const Token token(a, row, z);
+  float x[NV * VEC];
+#pragma unroll
+  for (int k = 0; k < NV; ++k) {
+    const int c = k * kAcross + l * VEC;
+    if (c + VEC <= V) {
+      const Vec<E, VEC> r = vload<E, VEC>(z + c);
+#pragma unroll
+      for (int v = 0; v < VEC; ++v) x[k * VEC + v] = (float)r.v[v];
+    } else {
+#pragma unroll
+      for (int v = 0; v < VEC; ++v) x[k * VEC + v] = c + v < V ? (float)z[c + v] : -INFINITY;
+    }
+  }
+  Sums t;
+#pragma unroll
+  for (int i = 0; i < NV * VEC; ++i) t.m = fmaxf(t.m, x[i]);
+  t.m = max16(t.m);
+  const float mm = t.m == -INFINITY ? 0.0f : t.m;
+  float below = 0.0f;
+#pragma unroll
+  for (int i = 0; i < NV * VEC; ++i) {
+    const float d = __builtin_elementwise_maximum(x[i] - mm, kFar);  // (a NaN passes)
+    const float e = __expf(d);
+    const float less = __builtin_amdgcn_fmed3f(d * -0x1p126f, 0.0f, 1.0f);  // 0 at m, else 1
+    t.s = fmaf(e, less, t.s);
+    below += less;
+    t.u = fmaf(e, d, t.u);
+  }
+  auto plus = [](float p, float q) { return p + q; };
+  t.s = reduce16(t.s, plus);
+  t.u = reduce16(t.u, plus);
+  t.c = NV * kAcross - reduce16(below, plus);
+  const RowStats st(t);
+  if (l == 0 && at < a.N) finish_row(a, row, st, token);
+  if (TOP) {
+    __shared__ u64 cand[16][kShortCand];
+    select_short<E>(cand[threadIdx.x >> 4], a.top, x, z, V, at < a.N,
+                    [&](int r, u64 key) { emit_top(a, row, r, key, st); });
+  }
+}
+
 // One workgroup a row: the first wave joins the segments' statistics (a lane a segment); of the
-// segments' lists the keys that can be among the first `top` are ranked.
+// segments' lists the keys that can be among the first `top` are ranked.  5 rows of 151001 fp16 classes
+// with 20 alternatives: 9 us for the segments and 5 for this, both chains of a few dependent steps.
 template <typename E>
 __global__ __launch_bounds__(256) void class_probs_join_kernel(ProbArgs a) {
   const long row = blockIdx.x;
@@ -500,8 +687,9 @@ __global__ __launch_bounds__(256) void class_probs_join_kernel(ProbArgs a) {
   rank_out<256>(cand, count, tid, a.top, [&](int r, u64 k) { emit_top(a, row, r, k, t); });
 }
 
-// dz = dlogp (onehot - p) - dentropy p ((z - m) + mean): one read, one write.  1 - p of the largest
-// class is rest / (1 + rest).
+// dz = dlogp (onehot - p) - dentropy p ((z - m) + mean): one read, one write, and bound by them (4096
+// rows of 50001 bf16 classes 175 us, 4.7 TB/s); a wave takes two vectors a lane of a row, so the rows'
+// lengths do not matter to the balance.  1 - p of the largest class is rest / (1 + rest).
 template <typename E>
 __global__ __launch_bounds__(256) void class_probs_backward_kernel(ProbArgs a, const float* dlogp,
                                                                    const float* dentropy, void* dz, long lddz,
@@ -553,6 +741,9 @@ __global__ __launch_bounds__(256) void class_probs_backward_kernel(ProbArgs a, c
 }
 
 
+// (fewer rows than 4096 take 5 to 7 us either way)
+bool short_rows(long N, long V) { return V <= kShort && N >= 4096; }
+
 // A wave takes a row where rows are short, or many enough to fill the chip so (4096 rows of 50001
 // bf16 classes: 83 us, with a workgroup a row 90); else a workgroup does.
 bool wave_rows(long N, long V) { return V <= 2048 || N >= 4096; }
@@ -590,6 +781,15 @@ int check_rows(int dtype, long N, long V, long ldz) {
 
 template <typename E, bool TOP>
 int run_forward(ProbArgs a, hipStream_t s) {
+  if (short_rows(a.N, a.V)) {
+    constexpr int most = kShort / 16 / width<E>();  // vectors a lane
+    const unsigned grid = (unsigned)((a.N + 15) / 16);
+    if (a.V <= kShort / 4) class_probs_short_kernel<E, most / 4, TOP><<<grid, 256, 0, s>>>(a);
+    else if (a.V <= kShort / 2) class_probs_short_kernel<E, most / 2, TOP><<<grid, 256, 0, s>>>(a);
+    else class_probs_short_kernel<E, most, TOP><<<grid, 256, 0, s>>>(a);
+    AVC_LAUNCH_CHECK();
+    return AVC_OK;
+  }
   if (wave_rows(a.N, a.V)) {
     class_probs_forward_kernel<E, 64, TOP><<<(unsigned)((a.N + 3) / 4), 256, 0, s>>>(a);
     AVC_LAUNCH_CHECK();

@@ -188,6 +188,10 @@ __device__ void join_segments(const RecArgs& a, int lo, int hi, const float* agg
   __syncthreads();
 }
 
+// A workgroup walks its segment chunk by chunk: each wave forms its stretch's action from gates that were
+// asked for a chunk earlier, the actions meet in LDS (double-buffered: one barrier a chunk), and each
+// wave goes over its own stretch, still in registers, with the state that comes to it.  Gates are read
+// once and y written once: 128x256x512 fp32 55 us (4.9 TB/s, the rate of a large copy), bf16 31 us.
 template <typename E, int VEC, bool RAGGED>
 __global__ __launch_bounds__(kW * 64, 4) void recurrence_forward_kernel(RecArgs a) {
   constexpr int kS = stretch<VEC, false>(), kChunk = kS * kW;
@@ -278,6 +282,10 @@ __global__ __launch_bounds__(kW * 64, 4) void recurrence_forward_kernel(RecArgs 
   if (a.hT && last == (a.T + kChunk - 1) / kChunk && wave == 0 && at.ok) give<VEC>(a.hT + st0, soff, h);
 }
 
+// The same walk from the last chunk to the first, with the action on the state too (from the state kept
+// at the chunk's beginning), so that h needs no pass of its own.  Bound by reading gates and dy and
+// writing dgates once: 128x256x512 fp32 102 us (4.6 TB/s; 87 right behind the forward, which leaves some
+// of the gates in the last-level cache), bf16 48 us.
 template <typename E, int VEC, bool RAGGED>
 __global__ __launch_bounds__(kW * 64, 2) void recurrence_backward_kernel(RecArgs a) {
   constexpr int kS = stretch<VEC, true>(), kChunk = kS * kW;
@@ -420,7 +428,9 @@ __global__ __launch_bounds__(kW * 64, 2) void recurrence_backward_kernel(RecArgs
 }
 
 // What one segment of time does to the state before it (BACK: to the gradient behind it): each
-// wave walks a run of stretches of its own, then the waves' runs are joined in order.
+// wave walks a run of stretches of its own, then the waves' runs are joined in order.  It reads two
+// thirds of the gates (60001x1x500 fp16: 36 us, then 57 us for the forward).  One pass in which the
+// workgroups hand the state on as they go read them once and took longer: 137 us instead of 111 then.
 template <typename E, int VEC, bool RAGGED, bool BACK>
 __global__ __launch_bounds__(kW * 64, 6) void recurrence_segment_kernel(RecArgs a) {
   constexpr int kS = 16;  // frames in flight (with 4 the ragged backward's took 17 us, with 16 it takes 15)
@@ -499,7 +509,7 @@ __global__ __launch_bounds__(kW * 64, 6) void recurrence_segment_kernel(RecArgs 
   }
 }
 
-// One frame of every row: the served form.
+// One frame of every row: the served form.  Bound by its launch (512 channels 1.9 us).
 template <typename E, int VEC>
 __global__ __launch_bounds__(256) void recurrence_step_kernel(int B, int H, const E* gates, long ldg, const float* h,
                                                               float* h_out, E* y, long ldy) {

@@ -111,9 +111,9 @@ def log_softmax(z):
 
 
 def entropy_of(lp):
-    """Of log-probabilities along the last dimension (0 log 0 = 0)."""
+    """Of log-probabilities along the last dimension (0 log 0 = 0; a NaN makes it NaN)."""
     p = torch.exp(lp)
-    return -torch.where(p > 0, p * lp, torch.zeros_like(p)).sum(-1)
+    return -torch.where(p == 0, torch.zeros_like(p), p * lp).sum(-1)
 
 
 def log_probs(logits, tokens, top=0, ignore_index=-100):

@@ -279,6 +279,63 @@ def test_log_probs(cuda_device, dtype, N, V, top, masked):
 
 
 @pytest.mark.parametrize("dtype", TYPES, ids=IDS)
+@pytest.mark.parametrize("N,V,top", [
+    (4096, 1, 1), (4097, 7, 0), (4099, 40, 32), (4100, 128, 9), (4111, 129, 0), (4096, 256, 16), (4101, 257, 5), (4096, 300, 8),
+    (4098, 512, 20), (4096, 511, 32), (4097, 513, 3)])
+@pytest.mark.parametrize("masked", [False, True])
+def test_log_probs_many_short_rows(cuda_device, dtype, N, V, top, masked):
+    gen = torch.Generator().manual_seed(N * V + top)
+    z = _logits(gen, N, V, dtype, masked)
+    tok = torch.randint(0, V, (N,), generator=gen)
+    tok[0], tok[3] = -100, -100
+    _check_log_probs(cuda_device, z, tok, top)
+
+
+@pytest.mark.parametrize("top", [0, 1, 8, 16, 32])
+def test_log_probs_many_short_rows_of_every_kind(cuda_device, top):
+    """Neighbouring rows that share a wave and need different things: equal classes, fewer classes left
+    than are wanted, none, the largest classes side by side or rising, NaN and infinity, confident rows."""
+    N, V = 4099, 500
+    gen = torch.Generator().manual_seed(top)
+    z = torch.randn(N, V, generator=gen)
+    z[1::11] = 0.25
+    z[2::11] = torch.randint(0, 3, (len(z[2::11]), V), generator=gen).float()
+    z[3::11, 5:] = -math.inf
+    z[4::11] = -math.inf
+    z[5::11] = torch.linspace(-4, 4, V)
+    for c in range(8):  # the classes that one lane of 16 holds in fours
+        z[6::11, 24 + 64 * c:min(28 + 64 * c, V)] += 9.0
+    z[7::11] = torch.where(torch.rand(len(z[7::11]), V, generator=gen) < 0.97, torch.tensor(-math.inf), z[7::11])
+    z[8::11, 100] = 25.0
+    z[9::11, 3] = -0.0
+    z[9::11, 2] = 0.0
+    z[9::11, 4:] = -1.0
+    tok = torch.randint(0, V, (N,), generator=gen)
+    _check_log_probs(cuda_device, z, tok, top)
+    z[10::11, 7] = math.nan
+    z[21::11, 400] = math.inf
+    tok[::5], tok[1::5] = V, -1
+    logp, H, tl, ti = so.log_probs(z, tok, top)
+    got = ops.token_log_probs(z.to(cuda_device), tok.to(cuda_device), top=top)
+    assert torch.equal(torch.isnan(got[0].cpu()), torch.isnan(logp)) and torch.equal(torch.isnan(got[1].cpu()), torch.isnan(H))
+    assert torch.equal(got[3].cpu(), ti) and torch.equal(torch.isnan(got[2].cpu()), torch.isnan(tl))
+
+
+def test_log_probs_of_many_confident_short_rows(cuda_device):
+    """As test_log_probs_of_confident_rows: 64 classes a lane at most and four joins."""
+    N, V = 4096, 400
+    gen = torch.Generator().manual_seed(V)
+    z = torch.randn(N, V, generator=gen)
+    top = torch.randint(0, V, (N,), generator=gen)
+    z[torch.arange(N), top] = z.max() + torch.linspace(2.0, 22.0, N) + math.log(V)
+    logp, H, _, _ = so.log_probs(z, top)
+    got = ops.token_log_probs(z.to(cuda_device), top.to(cuda_device))
+    rel = 350 * so.U
+    _near(got[0], logp, rel * logp.abs(), "logp")
+    _near(got[1], H, rel * H, "entropy")
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS)
 def test_log_probs_ties_go_to_the_lower_class(cuda_device, dtype):
     for V in (40, 512, 3001, 50001):
         z = torch.zeros(3, V, dtype=dtype)
