@@ -53,9 +53,9 @@ __device__ __forceinline__ void drop_vec(const DropArgs& a, unsigned long long k
 }
 
 // Bound by its reads and the write: 65536x1024 bf16 with a residual 83 us (4.9 TB/s, the rate of a large
-// copy), its gradient 58 us (4.6 TB/s).  A thread takes kUnroll vectors; a row's last vector is moved back to end at the row's end (the
-// elements it shares with its neighbour get the same value twice), so none is cut unless the row
-// is shorter than one.  FLAT: the rows follow one another and are taken as one.
+// copy), its gradient 58 us (4.6 TB/s).  A thread takes kUnroll vectors; a row's last vector is moved
+// back to end at the row's end (the elements it shares with its neighbour get the same value twice), so
+// none is cut unless the row is shorter than one.  FLAT: the rows follow one another and are taken as one.
 template <typename E, bool FLAT, bool RES>
 __global__ __launch_bounds__(256) void dropout_kernel(DropArgs a) {
   constexpr int VEC = width<E>();

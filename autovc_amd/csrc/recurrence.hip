@@ -429,7 +429,7 @@ __global__ __launch_bounds__(kW * 64, 2) void recurrence_backward_kernel(RecArgs
 
 // What one segment of time does to the state before it (BACK: to the gradient behind it): each
 // wave walks a run of stretches of its own, then the waves' runs are joined in order.  It reads two
-// thirds of the gates (60001x1x500 fp16: 36 us, then 57 us for the forward).  One pass in which the
+// thirds of the gates (60001x1x500 fp16: 36 us, then 60 us for the forward).  One pass in which the
 // workgroups hand the state on as they go read them once and took longer: 137 us instead of 111 then.
 template <typename E, int VEC, bool RAGGED, bool BACK>
 __global__ __launch_bounds__(kW * 64, 6) void recurrence_segment_kernel(RecArgs a) {
