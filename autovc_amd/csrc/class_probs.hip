@@ -12,6 +12,7 @@
 // (a class elsewhere has k classes above it), so only those slices are read again.
 // Classes are ordered by one 64-bit key, the value's bits made monotone above the complement of
 // the class number: larger values first, equal ones by the lower class, no two keys alike.
+#include <algorithm>
 #include <climits>
 #include <utility>
 
@@ -774,8 +775,24 @@ size_t probs_workspace(long N, long V, int top, int vec) {
 int check_rows(int dtype, long N, long V, long ldz) {
   AVC_CHECK_ARG(dtype_ok(dtype), "dtype is one of AVC_DTYPE_F32, _BF16, _F16");
   AVC_CHECK_ARG(N >= 0 && V >= 1, "N >= 0, V >= 1");
-  AVC_CHECK_ARG(V <= 1L << 30 && N < 1L << 24, "N or V too large");
+  AVC_CHECK_ARG(V <= 1L << 30 && N <= 1L << 40, "N or V too large");
   AVC_CHECK_ARG(ldz >= V, "a row stride is smaller than V");
+  return AVC_OK;
+}
+
+// More rows than a grid takes go in launches of nearly equal parts, each with rows enough for the whole's
+// layout.  (a is the part: its first row and number of rows set)
+template <typename E, typename Launch>
+int in_parts(const ProbArgs& all, long most, Launch launch) {
+  const long parts = (all.N + most - 1) / most, per = (all.N + parts - 1) / parts;
+  for (long r = 0; r < all.N; r += per) {
+    ProbArgs a = all;
+    a.N = std::min(per, all.N - r);
+    a.z = static_cast<const E*>(all.z) + r * all.ldz;
+    a.tokens = all.tokens + r;
+    if (all.stats) a.stats = all.stats + r * 3;
+    AVC_TRY(launch(a, r));
+  }
   return AVC_OK;
 }
 
@@ -836,7 +853,11 @@ extern "C" int avc_token_log_probs_forward(int dtype, long N, long V, const void
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   return with_dtype(dtype, [&](auto e) {
     using E = decltype(e);
-    return top ? run_forward<E, true>(a, s) : run_forward<E, false>(a, s);
+    return in_parts<E>(a, 1L << 23, [&](ProbArgs part, long r) {
+      part.logp += r, part.entropy += r;
+      if (top) part.top_logp += r * top, part.top_ids += r * top;
+      return top ? run_forward<E, true>(part, s) : run_forward<E, false>(part, s);
+    });
   });
 }
 
@@ -855,10 +876,12 @@ extern "C" int avc_token_log_probs_backward(int dtype, long N, long V, const voi
   return with_dtype(dtype, [&](auto e) {
     using E = decltype(e);
     const long tile = 64L * width<E>() * 2, tiles = (V + tile - 1) / tile;
-    AVC_CHECK_ARG(N <= (1L << 25) / tiles, "N * V too large");
-    class_probs_backward_kernel<E><<<(unsigned)((N * tiles + 3) / 4), 256, 0, s>>>(a, dlogp, dentropy, dlogits, lddz,
-                                                                                 (unsigned)tiles);
-    AVC_LAUNCH_CHECK();
-    return AVC_OK;
+    return in_parts<E>(a, (1L << 25) / tiles, [&](const ProbArgs& part, long r) {
+      class_probs_backward_kernel<E><<<(unsigned)((part.N * tiles + 3) / 4), 256, 0, s>>>(
+          part, dlogp ? dlogp + r : nullptr, dentropy ? dentropy + r : nullptr, static_cast<E*>(dlogits) + r * lddz, lddz,
+          (unsigned)tiles);
+      AVC_LAUNCH_CHECK();
+      return AVC_OK;
+    });
   });
 }

@@ -433,6 +433,28 @@ def test_log_probs_shapes_and_gradients_of_one_output(cuda_device):
     assert e[0].shape == (0,) and e[3].shape == (0, 2)
 
 
+@pytest.mark.parametrize("V", [3, 600])
+def test_log_probs_of_more_rows_than_a_launch_takes(cuda_device, V):
+    """Rows go in several launches: every row has what it has in a call of its neighbours alone."""
+    N = 2 ** 25 + 11
+    z = torch.empty(N, V, dtype=torch.float16, device=cuda_device)
+    z.normal_(generator=torch.Generator(device=cuda_device).manual_seed(9)).requires_grad_(True)
+    tok = torch.arange(N, device=cuda_device) % V
+    got = ops.token_log_probs(z, tok, top=2)
+    gl = torch.linspace(-1, 1, N, device=cuda_device)
+    dz, = torch.autograd.grad((got[0], got[1]), z, (gl, gl.flip(0)))
+    edges = [-(-N // -(-N // most)) for most in (2 ** 23, 2 ** 25)]  # the first parts' ends, forward and backward
+    for lo in (0, edges[0] - 2500, edges[1] - 2500, N - 5000):
+        rows = slice(lo, lo + 5000)
+        part = z.detach()[rows].clone().requires_grad_(True)
+        want = ops.token_log_probs(part, tok[rows], top=2)
+        for a, b in zip(got, want):
+            assert torch.equal(a[rows], b)
+        d, = torch.autograd.grad(want[:2], part, (gl[rows], gl.flip(0)[rows]))
+        assert torch.equal(dz[rows], d)
+    assert bool((got[0] <= 0).all()) and bool((got[1] > 0).all())
+
+
 def test_log_probs_past_32_bit_offsets(cuda_device):
     N, V = 45_000, 50_001
     z = torch.empty(N, V, dtype=torch.bfloat16, device=cuda_device)

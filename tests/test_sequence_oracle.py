@@ -118,7 +118,7 @@ def test_recurrence_step_refusals():
 
 @pytest.mark.parametrize("change", [
     dict(dtype=7), dict(N=-1), dict(V=0), dict(ldz=9), dict(top=-1), dict(top=33), dict(top=11), dict(z=None), dict(tok=None),
-    dict(top=2, topv=None), dict(N=1 << 24), dict(V=(1 << 30) + 1, ldz=1 << 31)])
+    dict(top=2, topv=None), dict(N=(1 << 40) + 1), dict(V=(1 << 30) + 1, ldz=1 << 31)])
 def test_log_probs_forward_refusals(change):
     a = dict(dtype=0, N=4, V=10, z=P, ldz=10, tok=P, top=0, topv=P) | change
     _refused("avc_token_log_probs_forward", a["dtype"], a["N"], a["V"], a["z"], a["ldz"], a["tok"], -100, a["top"], P, P, None,
