@@ -321,6 +321,19 @@ def test_log_probs_many_short_rows_of_every_kind(cuda_device, top):
     assert torch.equal(got[3].cpu(), ti) and torch.equal(torch.isnan(got[2].cpu()), torch.isnan(tl))
 
 
+@pytest.mark.parametrize("top", [8, 16, 32])
+def test_log_probs_many_short_rows_with_their_classes_in_few_lanes(cuda_device, top):
+    """More classes left than a row's list holds, all in three of its 16 lanes, beside rows with none
+    ruled out."""
+    N, V = 4096, 512
+    gen = torch.Generator().manual_seed(top)
+    z = torch.randn(N, V, generator=gen)
+    lane = torch.arange(V) // 4 % 16
+    z[1::3] = torch.where((lane >= 1) & (lane <= 3), z[1::3], torch.tensor(-math.inf))
+    z[5::9] = torch.where(lane == 9, z[5::9].round(), z[5::9] - 20.0)
+    _check_log_probs(cuda_device, z, torch.randint(0, V, (N,), generator=gen), top)
+
+
 def test_log_probs_of_many_confident_short_rows(cuda_device):
     """As test_log_probs_of_confident_rows: 64 classes a lane at most and four joins."""
     N, V = 4096, 400
