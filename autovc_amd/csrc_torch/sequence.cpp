@@ -288,8 +288,8 @@ LogProbs log_probs_forward(const Tensor& logits, const Tensor& tokens, long top,
   const long N = logits.size(0), V = logits.size(1);
   const Rows z(logits);
   const auto f32 = logits.options().dtype(at::kFloat);
-  LogProbs o{at::empty({N}, f32), at::empty({N}, f32), at::empty({N, top}, f32),
-             at::empty({N, top}, f32.dtype(at::kLong)), Tensor()};
+  LogProbs o{at::empty({N}, f32), at::empty({N}, f32), Tensor(), Tensor(), Tensor()};
+  if (top || !keep) o.top_logp = at::empty({N, top}, f32), o.top_ids = at::empty({N, top}, f32.dtype(at::kLong));
   if (keep) o.stats = at::empty({N, 3}, f32);
   if (N) {
     const size_t bytes = lib.avc_token_log_probs_workspace(dt, N, V, top);
@@ -308,8 +308,9 @@ struct TokenLogProbs : torch::autograd::Function<TokenLogProbs> {
     LogProbs o = log_probs_forward(logits, tokens, top, ignore, true);
     ctx->save_for_backward({logits, tokens, o.stats});
     ctx->saved_data["ignore"] = ignore;
-    ctx->mark_non_differentiable({o.top_logp, o.top_ids});
     ctx->set_materialize_grads(false);
+    if (!top) return {o.logp, o.entropy};
+    ctx->mark_non_differentiable({o.top_logp, o.top_ids});
     return {o.logp, o.entropy, o.top_logp, o.top_ids};
   }
   static variable_list backward(AutogradContext* ctx, variable_list d) { return once(d, grads(ctx, d)); }
@@ -339,14 +340,20 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> token_log_probs(Tensor logits, Tensor
                     "logits [..., V >= 1] and tokens [...] must agree, got ", logits.sizes(), " and ", tokens.sizes());
   const long V = logits.size(-1), most = std::min<long>(32, V);
   TORCH_CHECK_VALUE(top >= 0 && top <= most, "top must be 0 .. ", most, ", got ", top);
-  tokens = tokens.to(at::kLong).contiguous();
+  if (tokens.scalar_type() != at::kLong) tokens = tokens.to(at::kLong);
+  if (!tokens.is_contiguous()) tokens = tokens.contiguous();
   const auto lead = tokens.sizes().vec();
   const bool flat = logits.dim() == 2;
   if (!flat) logits = logits.reshape({tokens.numel(), V}), tokens = tokens.reshape({-1});
   Tensor logp, entropy, tl, ti;
   if (wants_grad(logits)) {
     auto o = TokenLogProbs::apply(logits, tokens, top, ignore);
-    logp = o[0], entropy = o[1], tl = o[2], ti = o[3];
+    logp = o[0], entropy = o[1];
+    if (top) {
+      tl = o[2], ti = o[3];
+    } else {
+      tl = at::empty({tokens.numel(), 0}, logp.options()), ti = at::empty({tokens.numel(), 0}, tokens.options());
+    }
   } else {
     LogProbs o = log_probs_forward(logits, tokens, top, ignore, false);
     logp = o.logp, entropy = o.entropy, tl = o.top_logp, ti = o.top_ids;
