@@ -750,9 +750,9 @@ bool short_rows(long N, long V) { return V <= kShort && N >= 4096; }
 bool wave_rows(long N, long V) { return V <= 2048 || N >= 4096; }
 
 // Segments of a row: where there are few long rows (below 16 rounds of a workgroup the second launch
-// costs more than it gives: 64 rows of 8192 fp32 classes 15.0 us cut, 11.4 whole) each is cut until
-// the chip is full, into pieces of two rounds at least (5 rows of 151001 fp16 classes with 20
-// alternatives: pieces of two rounds 15.6 us, of four 22.3, of eight 17.2).
+// costs more than it gives: 64 rows of 8192 fp32 classes 8.3 us cut, 5.3 whole) each is cut until the
+// chip is full, into pieces of two rounds at least (5 rows of 151001 fp16 classes with 20 alternatives:
+// pieces of two rounds 14.0 us, of four 21.9, of eight 20.5; without alternatives 8 us each way).
 int row_segments(long N, long V, int vec, long* seg) {
   *seg = V;
   const long round = 256L * vec;
