@@ -557,7 +557,8 @@ __global__ __launch_bounds__(256) void recurrence_step_kernel(int B, int H, cons
 }
 
 // Channels of a lane: 4 bytes.  (8-byte lanes hold twice the registers: a training pass of
-// 128x256x512 took 60 + 106 us in fp32 instead of 53 + 101, 37 + 142 us in bf16 instead of 32 + 57.)
+// 128x256x512 takes 89 + 98 us in fp32 instead of 55 + 102, 76 + 55 us in bf16 instead of 31 + 48;
+// 2-byte lanes of 16-bit gates 37 + 55.)
 template <typename E>
 constexpr int wide() { return sizeof(E) == 4 ? 1 : 2; }
 
@@ -565,7 +566,8 @@ constexpr int wide() { return sizeof(E) == 4 ? 1 : 2; }
 // enough to fill the chip each workgroup walks its rows' whole time; with fewer, time is cut into as
 // many segments as bring the grid to two workgroups a CU, which costs a pass over most of the gates
 // for the segments' actions and a launch.  1024 frames in 128 tiles (bf16, ragged): cut in four
-// 42 us, whole 57; 60001 frames in 4 tiles: 128 segments 100 us, 64 111.  Up to 512 frames are not
+// 42 us, in two 49, whole 57; 60001 frames in 4 tiles: 128 segments 93 us, 64 106; twice as many segments
+// 43 and, in launch order, 107 (128: 100).  Up to 512 frames are not
 // cut: 400 frames in 180 tiles 36 us cut, 26 whole; 200 frames in 16 tiles 13 us either way.
 struct Layout {
   int log_g = 0, nct, nseg, seg_chunks;
