@@ -462,7 +462,8 @@ __global__ __launch_bounds__(GT * kRows<GT>) void class_probs_forward_kernel(Pro
 // which spares three quarters of what a row costs beside its classes (reductions, logarithms) -- with
 // a wave a row that is what bounds it.  35200 rows of 512 fp32 classes 14.6 us (4.9 TB/s, the rate of a
 // large copy), with a wave a row 19.9; with 5 alternatives 26 and 38; 60000 rows of 100 fp32 classes with
-// 5 alternatives 18 and 57.  (Up to 20 alternatives it is never slower there; 32 of 512 classes 47 and 45.)
+// 5 alternatives 18 and 57.  (Many alternatives of 512
+// fp32 classes are the exception: 35200 rows with 32 47 and 45, 4096 with 20 11 and 9.)
 constexpr int kShort = 512;
 constexpr int kShortCand = 64;  // candidates of a row that are ranked at once
 
