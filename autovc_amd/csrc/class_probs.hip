@@ -141,8 +141,9 @@ struct Sums {
   __device__ __forceinline__ void join_wave() {
     s = wave_sum(s);
     u = wave_sum(u);
-    // mostly one lane holds the one class at m
-    c = __any(c > 1.0f) ? wave_sum(c) : (float)__popcll(__ballot(c == 1.0f));
+    // Mostly one lane holds the one class at m.  (c is no whole number where a class lies less than 2^-126
+    // below m: `less` is a part of 1 then, and s and c hold such a class's term together.)
+    c = __any(c != 0.0f && c != 1.0f) ? wave_sum(c) : (float)__popcll(__ballot(c == 1.0f));
   }
 };
 
