@@ -98,6 +98,12 @@ void check_type(const Tensor& t, const char* name, const Tensor& like, at::Scala
   TORCH_CHECK_TYPE(t.scalar_type() == a || t.scalar_type() == b, name, " has dtype ", t.scalar_type());
 }
 
+// A tangent of forward-mode differentiation would be lost: the outputs are filled behind torch's back.
+template <typename... T>
+void check_tangents(const char* what, const T&... inputs) {
+  TORCH_CHECK((... && !torch::autograd::isFwGradDefined(inputs)), what, " has no forward-mode derivative");
+}
+
 // A matrix whose rows the kernels can walk: t itself unless its rows are not dense or overlap.
 struct Rows {
   Tensor t;
@@ -202,6 +208,7 @@ struct GatedRecurrence : torch::autograd::Function<GatedRecurrence> {
 
 std::tuple<Tensor, Tensor> gated_recurrence(const Tensor& gates, long T, long B, optional<Tensor> h0, optional<Tensor> lengths,
                                             long dirs) {
+  check_tangents("gated_recurrence", gates, h0);
   check_data(gates, "gates");
   TORCH_CHECK_VALUE(dirs >= 1 && dirs <= 3, "dirs is 1 (forward), 2 (reverse) or 3 (both)");
   const long D = dirs == 3 ? 2 : 1, most = 1L << 30;
@@ -244,6 +251,7 @@ bool overlap(const Tensor& a, const Tensor& b) {
 }
 
 std::tuple<Tensor, Tensor> gated_recurrence_step(const Tensor& gates, const Tensor& state, optional<Tensor> out_state) {
+  check_tangents("gated_recurrence_step", gates, state, out_state);
   check_data(gates, "gates");
   check_type(state, "state", gates, at::kFloat, at::kFloat);
   TORCH_CHECK_VALUE(gates.dim() == 2 && gates.size(1) > 0 && gates.size(1) % 3 == 0, "gates must be [B][3 * H], got ",
@@ -334,6 +342,7 @@ struct TokenLogProbs : torch::autograd::Function<TokenLogProbs> {
 };
 
 std::tuple<Tensor, Tensor, Tensor, Tensor> token_log_probs(Tensor logits, Tensor tokens, long top, long ignore) {
+  check_tangents("token_log_probs", logits);
   check_data(logits, "logits");
   check_type(tokens, "tokens", logits, at::kLong, at::kInt);
   TORCH_CHECK_VALUE(logits.dim() >= 1 && logits.size(-1) >= 1 && logits.sizes().slice(0, logits.dim() - 1) == tokens.sizes(),
@@ -411,6 +420,7 @@ struct Dropout : torch::autograd::Function<Dropout> {
 };
 
 Tensor dropout(const Tensor& x, double p, const Tensor& rng, optional<Tensor> residual, long layer) {
+  check_tangents("dropout", x, residual);
   check_data(x, "x");
   check_type(rng, "rng", x, at::kLong, at::kLong);
   TORCH_CHECK_VALUE(p >= 0.0 && p < 1.0, "p must be 0 <= p < 1, got ", p);

@@ -1,0 +1,28 @@
+"""CPU: what the sequence-model operators' torch functions refuse before they look for a GPU."""
+import pytest
+import torch
+import torch.autograd.forward_ad as fwd
+
+from autovc_amd import ops
+
+CALLS = {
+    "gated_recurrence": lambda x: ops.gated_recurrence(x, 2, 2)[0],
+    "gated_recurrence of h0": lambda x: ops.gated_recurrence(torch.zeros(4, 18), 2, 2, h0=x.reshape(1, 4, 6)[:, :2])[1],
+    "gated_recurrence_step": lambda x: ops.gated_recurrence_step(x, torch.zeros(4, 2))[0],
+    "gated_recurrence_step of its state": lambda x: ops.gated_recurrence_step(torch.zeros(4, 18), x)[1],
+    "token_log_probs": lambda x: ops.token_log_probs(x, torch.zeros(4, dtype=torch.int64))[0],
+    "dropout": lambda x: ops.dropout(x, 0.5, torch.zeros(2, dtype=torch.int64)),
+    "dropout of a residual": lambda x: ops.dropout(torch.zeros(4, 6), 0.5, torch.zeros(2, dtype=torch.int64), residual=x),
+}
+
+
+@pytest.mark.parametrize("call", CALLS.values(), ids=CALLS.keys())
+@pytest.mark.parametrize("grad", [False, True])
+def test_tangents_are_refused(call, grad):
+    """No derivative is dropped in silence, whether reverse mode is on beside it or not."""
+    with fwd.dual_level():
+        x = torch.zeros(4, 6, requires_grad=grad)
+        with pytest.raises(RuntimeError, match="no forward-mode derivative"):
+            call(fwd.make_dual(x, torch.ones(4, 6)))
+    with pytest.raises(RuntimeError, match="no forward-mode derivative"):
+        torch.func.jvp(call, (torch.zeros(4, 6),), (torch.ones(4, 6),))
