@@ -9,11 +9,13 @@
 // The library is the one that autovc_amd._lib has loaded: bind() is given its path.
 #include <ATen/ATen.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPStream.h>
 #include <dlfcn.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/functions/utils.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/extension.h>
 
 #include <algorithm>
@@ -98,10 +100,16 @@ void check_type(const Tensor& t, const char* name, const Tensor& like, at::Scala
   TORCH_CHECK_TYPE(t.scalar_type() == a || t.scalar_type() == b, name, " has dtype ", t.scalar_type());
 }
 
-// A tangent of forward-mode differentiation would be lost: the outputs are filled behind torch's back.
+// The outputs are filled behind torch's back: a tangent of forward-mode differentiation would be lost, and a
+// trace would hold nothing but the allocation of its outputs.
 template <typename... T>
-void check_tangents(const char* what, const T&... inputs) {
+void check_seen(const char* what, const T&... inputs) {
+  using Modes = c10::impl::TorchDispatchModeTLS;
+  using Mode = c10::impl::TorchDispatchModeKey;
   TORCH_CHECK((... && !torch::autograd::isFwGradDefined(inputs)), what, " has no forward-mode derivative");
+  TORCH_CHECK(!torch::jit::tracer::isTracing() && !Modes::get_mode(Mode::FAKE) && !Modes::get_mode(Mode::PROXY) &&
+                  !Modes::get_mode(Mode::FUNCTIONAL),
+              what, " cannot be traced: it is no operator of torch's dispatcher");
 }
 
 // A matrix whose rows the kernels can walk: t itself unless its rows are not dense or overlap.
@@ -208,7 +216,7 @@ struct GatedRecurrence : torch::autograd::Function<GatedRecurrence> {
 
 std::tuple<Tensor, Tensor> gated_recurrence(const Tensor& gates, long T, long B, optional<Tensor> h0, optional<Tensor> lengths,
                                             long dirs) {
-  check_tangents("gated_recurrence", gates, h0);
+  check_seen("gated_recurrence", gates, h0);
   check_data(gates, "gates");
   TORCH_CHECK_VALUE(dirs >= 1 && dirs <= 3, "dirs is 1 (forward), 2 (reverse) or 3 (both)");
   const long D = dirs == 3 ? 2 : 1, most = 1L << 30;
@@ -251,7 +259,7 @@ bool overlap(const Tensor& a, const Tensor& b) {
 }
 
 std::tuple<Tensor, Tensor> gated_recurrence_step(const Tensor& gates, const Tensor& state, optional<Tensor> out_state) {
-  check_tangents("gated_recurrence_step", gates, state, out_state);
+  check_seen("gated_recurrence_step", gates, state, out_state);
   check_data(gates, "gates");
   check_type(state, "state", gates, at::kFloat, at::kFloat);
   TORCH_CHECK_VALUE(gates.dim() == 2 && gates.size(1) > 0 && gates.size(1) % 3 == 0, "gates must be [B][3 * H], got ",
@@ -342,7 +350,7 @@ struct TokenLogProbs : torch::autograd::Function<TokenLogProbs> {
 };
 
 std::tuple<Tensor, Tensor, Tensor, Tensor> token_log_probs(Tensor logits, Tensor tokens, long top, long ignore) {
-  check_tangents("token_log_probs", logits);
+  check_seen("token_log_probs", logits);
   check_data(logits, "logits");
   check_type(tokens, "tokens", logits, at::kLong, at::kInt);
   TORCH_CHECK_VALUE(logits.dim() >= 1 && logits.size(-1) >= 1 && logits.sizes().slice(0, logits.dim() - 1) == tokens.sizes(),
@@ -420,7 +428,7 @@ struct Dropout : torch::autograd::Function<Dropout> {
 };
 
 Tensor dropout(const Tensor& x, double p, const Tensor& rng, optional<Tensor> residual, long layer) {
-  check_tangents("dropout", x, residual);
+  check_seen("dropout", x, residual);
   check_data(x, "x");
   check_type(rng, "rng", x, at::kLong, at::kLong);
   TORCH_CHECK_VALUE(p >= 0.0 && p < 1.0, "p must be 0 <= p < 1, got ", p);

@@ -7,7 +7,8 @@ column slices of a wider buffer (any row stride); other layouts are made contigu
 runs on the current stream of its tensors' device and allocates what it needs through torch, so it
 may be captured into a graph and used from several streams.  (A backward pass is captured only while no
 graph that was built outside the capture from the same leaves is alive, as torch asks for any of
-its own.)  Gradients are differentiable once; forward-mode derivatives are refused.
+its own.)  Gradients are differentiable once; forward-mode derivatives and
+tracing (torch.jit.trace, make_fx, fake tensors) are refused.
 Public names are re-exported by `autovc_amd.ops`.
 """
 from __future__ import annotations

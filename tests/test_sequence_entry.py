@@ -2,6 +2,8 @@
 import pytest
 import torch
 import torch.autograd.forward_ad as fwd
+from torch._subclasses import FakeTensorMode
+from torch.fx.experimental.proxy_tensor import make_fx
 
 from autovc_amd import ops
 
@@ -26,3 +28,15 @@ def test_tangents_are_refused(call, grad):
             call(fwd.make_dual(x, torch.ones(4, 6)))
     with pytest.raises(RuntimeError, match="no forward-mode derivative"):
         torch.func.jvp(call, (torch.zeros(4, 6),), (torch.ones(4, 6),))
+
+
+@pytest.mark.parametrize("call", CALLS.values(), ids=CALLS.keys())
+def test_traces_are_refused(call):
+    """A trace would hold the allocation of the outputs and not what fills them."""
+    with pytest.raises(RuntimeError, match="cannot be traced"):
+        torch.jit.trace(call, (torch.zeros(4, 6),), check_trace=False)
+    for mode in ("real", "fake"):
+        with pytest.raises(RuntimeError, match="cannot be traced"):
+            make_fx(call, tracing_mode=mode)(torch.zeros(4, 6))
+    with FakeTensorMode() as m, pytest.raises(RuntimeError, match="cannot be traced"):
+        call(m.from_tensor(torch.zeros(4, 6)))
