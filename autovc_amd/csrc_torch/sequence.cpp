@@ -144,14 +144,18 @@ bool wants_grad(const Tensor& a, const optional<Tensor>& b) {
 }
 
 // Gradients (formed without a graph) that are not differentiable themselves: where a graph of them is asked for
-// (create_graph), using that graph is an error.
-variable_list once(const variable_list& incoming, variable_list grads) {
+// (create_graph), using that graph is an error.  It leads to the incoming gradients and, unless the gradients
+// are linear in them alone, to the inputs of the running node.
+variable_list once(const variable_list& incoming, variable_list grads, bool linear = false) {
   if (!at::GradMode::is_enabled()) return grads;
-  const bool any = std::any_of(incoming.begin(), incoming.end(), [](const Tensor& g) { return g.defined() && g.requires_grad(); });
-  if (!any) return grads;
+  torch::autograd::edge_list edges = torch::autograd::collect_next_edges(incoming);
+  if (!linear) {
+    const auto& inputs = torch::autograd::get_current_node()->next_edges();
+    edges.insert(edges.end(), inputs.begin(), inputs.end());
+  }
+  if (std::none_of(edges.begin(), edges.end(), [](const auto& e) { return e.is_valid(); })) return grads;
   auto error = std::make_shared<torch::autograd::Error>(
-      "trying to differentiate twice a function whose gradient is not differentiable",
-      torch::autograd::collect_next_edges(incoming));
+      "trying to differentiate twice a function whose gradient is not differentiable", std::move(edges));
   for (Tensor& g : grads)
     if (g.defined()) torch::autograd::set_history(g, error);
   return grads;
@@ -417,7 +421,7 @@ struct Dropout : torch::autograd::Function<Dropout> {
   static variable_list backward(AutogradContext* ctx, variable_list d) {
     const long needs = ctx->saved_data["needs"].toInt();
     // (the residual's gradient is the incoming one itself, which keeps its own history)
-    return {needs & 1 ? once(d, {grad_x(ctx, d[0])})[0] : Tensor(), needs & 2 ? d[0] : Tensor(), Tensor(), Tensor(), Tensor()};
+    return {needs & 1 ? once(d, {grad_x(ctx, d[0])}, true)[0] : Tensor(), needs & 2 ? d[0] : Tensor(), Tensor(), Tensor(), Tensor()};
   }
   static Tensor grad_x(AutogradContext* ctx, const Tensor& dy) {
     // (rng is saved, so that changing it in place before the backward is an error and not another mask)

@@ -4,7 +4,8 @@ import math
 import pytest
 import torch
 
-from tests.test_gpu_sequence import _check_log_probs
+from autovc_amd import ops
+from tests.test_gpu_sequence import _check_log_probs, _rng
 
 pytestmark = pytest.mark.gpu
 
@@ -24,3 +25,24 @@ def test_log_probs_of_classes_a_subnormal_apart(cuda_device, dtype, N, V):
     tok = torch.randint(0, V, (N,), generator=gen)
     tok[:3] = torch.tensor([V // 2, 11, 5])
     _check_log_probs(cuda_device, z.to(dtype), tok, 4)
+
+
+def test_a_gradient_of_a_gradient_is_an_error(cuda_device):
+    """A penalty on a gradient, in whose graph nothing but the operator's own input needs a gradient."""
+    dev = cuda_device
+    g = torch.randn(12, 9, device=dev, requires_grad=True)
+    h0 = torch.randn(1, 2, 3, device=dev, requires_grad=True)
+    tok = torch.zeros(12, dtype=torch.int64, device=dev)
+    for out, leaf in ((ops.gated_recurrence(g, 6, 2)[0], g), (ops.gated_recurrence(g, 6, 2)[1], g),
+                      (ops.gated_recurrence(g.detach(), 6, 2, h0=h0)[0], h0),
+                      (ops.token_log_probs(g, tok)[0], g), (ops.token_log_probs(g, tok)[1], g)):
+        loss = out.sum()
+        d, = torch.autograd.grad(loss, leaf, create_graph=True)
+        with pytest.raises(RuntimeError, match="differentiate twice"):
+            (loss + d.square().sum()).backward()
+    # of a dropout the gradient does not depend on x: nothing is missing from the penalty's
+    loss = ops.dropout(g, 0.5, _rng(dev)).sum()
+    d, = torch.autograd.grad(loss, g, create_graph=True)
+    want, = torch.autograd.grad(ops.dropout(g, 0.5, _rng(dev)).sum(), g)
+    (loss + d.square().sum()).backward()
+    assert torch.equal(g.grad, want)
