@@ -57,18 +57,20 @@ __device__ __forceinline__ void forget_gate(float g, float& f, float& e) {
   e = __expf(-__builtin_elementwise_maximum(g, -80.0f));
   f = __builtin_amdgcn_rcpf(1.0f + e);
 }
-// tanh x = 1 - 2 / (1 + exp 2x).  fp32 gates take gate_tanh, whose error is a few units relative
-// everywhere.  For 16-bit ones a cubic below 1/32 and the formula above it do: the formula is off by
-// 6 * 2^-24 absolutely at most (two instructions of 1 unit, a sum and a rounded argument, on a
-// reciprocal <= 1/2 taken twice), which at 1/32 is 192 * 2^-24 of the value -- below 2^-16, a
-// sixteenth of the half step that an fp16 gate itself was rounded by -- and the cubic by
-// 2/15 x^4 < 2^-22; 5 instructions less a gate.
+// tanh of the candidate.  fp32 gates take gate_tanh; 16-bit ones, whose lanes form two a frame and feel every
+// instruction, the same with a shorter polynomial: a minimax one of x^7 below 0.35 (off by 0.7 units of
+// 2^-24 relative, 1.7 with its roundings), and above it 1 - 2 / (1 + exp 2|x|) with x's sign, whose error of
+// about 1 unit absolutely is 3 of the value there.  Over all bf16 and fp16 values either form is off by
+// 3.1 units at most: the state that a call hands to the next is fp32 whatever the gates' type.
+// (60001x1x500 fp16 forward 95 us, with gate_tanh 100; 1024x32x256 both directions ragged bf16 45 and 48.)
 template <typename E>
 __device__ __forceinline__ float candidate(float x) {
   if (sizeof(E) == 4) return gate_tanh(x);
-  const float small = fmaf(x * x, x * -0.333333333f, x);
-  const float big = fmaf(-2.0f, __builtin_amdgcn_rcpf(1.0f + __expf(2.0f * x)), 1.0f);
-  return fabsf(x) < 0.03125f ? small : big;
+  const float x2 = x * x, ax = fabsf(x);
+  const float p = fmaf(fmaf(x2, -0.0491485037f, 0.132998258f), x2, -0.333326638f);
+  const float small = fmaf(x * x2, p, x);
+  const float big = fmaf(-2.0f, __builtin_amdgcn_rcpf(1.0f + __expf(2.0f * ax)), 1.0f);
+  return ax < 0.35f ? small : copysignf(big, x);
 }
 
 // Where a lane works: VEC channels of one row b in one direction.  Rows narrower than a wave share

@@ -48,12 +48,7 @@ def recurrence_bounds(gates, T, B, h0=None, lengths=None, dirs=1, dy=None, dhT=N
     and reciprocal that follow, a gate is off by at most (|g| + 8) U relative (z and a gate's
     complement too: neither is formed by a subtraction that cancels).  C = max |g| + 12 leaves 4
     units for the products and sums of one frame, in whatever order the frames are joined: a
-    product of gates is off by the sum of its factors' relative errors, as it is frame by frame.
-
-    z of 16-bit gates: for |x| >= 1/32 it is 1 - 2 r with r = 1 / (1 + exp 2x) <= 1/2 (x > 0; the other
-    side is its mirror) off by (1 + 1 + 2) U for the reciprocal, the sum and the exponential with its
-    argument's rounding, so z by 6 U with its own rounding, 192 U of z >= 1/32; below, a cubic is off
-    by 2/15 x^4 < 3 U of z: CZ = C + 192 U holds for both."""
+    product of gates is off by the sum of its factors' relative errors, as it is frame by frame."""
     D = 2 if dirs == 3 else 1
     H = gates.shape[1] // (3 * D)
     g = gates.double().view(T, B, D, 3, H)
@@ -61,7 +56,6 @@ def recurrence_bounds(gates, T, B, h0=None, lengths=None, dirs=1, dy=None, dhT=N
     dead = torch.tensor([[t >= length[b] for b in range(B)] for t in range(T)]).view(T, B, 1, 1, 1)
     g = torch.where(dead, torch.zeros((), dtype=torch.float64), g)
     C = (min(g.abs().max().item(), 100.0) + 12) * U
-    CZ = C + (0 if gates.dtype in (torch.float32, torch.float64) else 192 * U)
     z0 = torch.zeros(T, B, D, H, dtype=torch.float64)
     f, i, z, o = torch.sigmoid(g[..., 0, :]), torch.sigmoid(-g[..., 0, :]), torch.tanh(g[..., 1, :]), torch.sigmoid(g[..., 2, :])
     dead = dead[..., 0]
@@ -78,7 +72,7 @@ def recurrence_bounds(gates, T, B, h0=None, lengths=None, dirs=1, dy=None, dhT=N
         for t in order:
             before[t], Eb[t] = h, E
             ft, it, zt = f[t, :, d], i[t, :, d], z[t, :, d]
-            E = ft * E + live[t, :, d] * (C * ft * h.abs() + CZ * it * zt.abs())
+            E = ft * E + live[t, :, d] * C * (ft * h.abs() + it * zt.abs())
             h = ft * h + it * zt
             after[t], Ea[t] = h, E
             Ey[t, :, d] = live[t, :, d] * (o[t, :, d] * E + C * (o[t, :, d] * h).abs())
@@ -91,8 +85,8 @@ def recurrence_bounds(gates, T, B, h0=None, lengths=None, dirs=1, dy=None, dhT=N
             Ee = Ec + C * ((ot * dyt).abs() + c.abs())
             dif = before[t] - zt
             # f (1 - f) and the like carry 2 C, a difference the errors of its operands
-            EdG[t, :, d, 0] = ft * it * (Ee * dif.abs() + e.abs() * (Eb[t] + C * before[t].abs() + CZ * zt.abs()) + 3 * C * (e * dif).abs())
-            EdG[t, :, d, 1] = it * (Ee * (1 - zt * zt) + e.abs() * (2 * CZ * zt * zt + 3 * C))
+            EdG[t, :, d, 0] = ft * it * (Ee * dif.abs() + e.abs() * (Eb[t] + C * (before[t].abs() + zt.abs())) + 3 * C * (e * dif).abs())
+            EdG[t, :, d, 1] = it * (Ee * (1 - zt * zt) + e.abs() * (2 * C * zt * zt + 3 * C))
             EdG[t, :, d, 2] = dyt.abs() * ot * (Ea[t] + 3 * C * after[t].abs())
             c = ft * e
             Ec = ft * Ee + C * live[t, :, d] * c.abs()

@@ -5,7 +5,8 @@ import pytest
 import torch
 
 from autovc_amd import ops
-from tests.test_gpu_sequence import _check_log_probs, _rng
+from oracle import sequence_oracle as so
+from tests.test_gpu_sequence import IDS, TYPES, _check_log_probs, _near, _rng
 
 pytestmark = pytest.mark.gpu
 
@@ -25,6 +26,24 @@ def test_log_probs_of_classes_a_subnormal_apart(cuda_device, dtype, N, V):
     tok = torch.randint(0, V, (N,), generator=gen)
     tok[:3] = torch.tensor([V // 2, 11, 5])
     _check_log_probs(cuda_device, z.to(dtype), tok, 4)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS)
+def test_recurrence_state_of_small_candidates(cuda_device, dtype):
+    """The fp32 state of one frame is as exact for 16-bit gates as for fp32 ones: with the forget gate at 1/2
+    the state is tanh(c) / 2, off by at most 16 units: the candidate's 12 (a reciprocal, a sum and an
+    exponential with its argument's rounding are off by 5.8, on 2 r = 0.66 of z = 0.34 where its two forms
+    meet, and its own rounding), the gate's 3 and the product's."""
+    steps = torch.arange(1, 64, dtype=torch.float64) / 64
+    c = torch.cat([2.0 ** e * (1 + steps) for e in range(-13, 1)]).to(dtype)
+    c = torch.cat([c, -c])
+    g = torch.zeros(1, 3, len(c), dtype=dtype)
+    g[0, 1] = c
+    want = torch.tanh(c.double()) / 2
+    y, hT = ops.gated_recurrence(g.view(1, -1).to(cuda_device), 1, 1)
+    _near(hT.flatten(), want, 16 * so.U * want.abs(), "hT")
+    y, state = ops.gated_recurrence_step(g.view(1, -1).to(cuda_device), torch.zeros(1, len(c), device=cuda_device))
+    _near(state.flatten(), want, 16 * so.U * want.abs(), "state")
 
 
 def test_a_gradient_of_a_gradient_is_an_error(cuda_device):
