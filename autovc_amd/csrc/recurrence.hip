@@ -49,6 +49,7 @@ struct RecArgs {
   int nseg, seg_chunks;
   int log_g, nct;    // lanes of a wave per row (log2), channel tiles per row
   unsigned pack;     // workgroups that are reordered among themselves (0: none)
+  unsigned tile0;    // first tile of the launch
 };
 
 // The forget gate as f = 1 / (1 + e), 1 - f = e f with e = exp(-g).  Below -80 (f < 2e-35) e is held
@@ -94,6 +95,7 @@ struct Place {
       bx = id % gx, id /= gx;
       seg = id % gy, d = id / gy;
     }
+    bx += a.tile0;
     wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     lane = threadIdx.x & 63;
     const int g = 1 << a.log_g;
@@ -598,7 +600,7 @@ int run_recurrence(RecArgs a, size_t ws_bytes, hipStream_t s) {
   a.log_g = l.log_g, a.nct = l.nct, a.nseg = l.nseg, a.seg_chunks = l.seg_chunks;
   const size_t need = l.workspace(a.B, a.H, D);
   AVC_CHECK_ARG(ws_bytes >= need && (need == 0 || a.agg), "workspace smaller than avc_gated_recurrence_workspace");
-  AVC_CHECK_ARG(l.tiles < (1L << 32) / (kW * 64), "B * H too large");
+  AVC_CHECK_ARG(l.tiles < 1L << 32, "B * H too large");
   // the rows that share a wave are reached by 32-bit offsets from the first of them
   const long widest = std::max(a.ldg, std::max(a.ldy, std::max(a.lddy, a.lddg)));
   AVC_CHECK_ARG(widest < (1L << 29) >> (6 - l.log_g), "row stride too large");
@@ -608,21 +610,27 @@ int run_recurrence(RecArgs a, size_t ws_bytes, hipStream_t s) {
   const long line = 128 / (long)sizeof(E);
   const bool split = a.H % line || a.ldg % line || reinterpret_cast<uintptr_t>(a.gates) % 128;
   a.pack = split && l.nct > 1 ? 8u * l.nct : 0;
-  const dim3 grid((unsigned)l.tiles, a.nseg, D);
-  if (a.nseg > 1) {
-    const dim3 before((unsigned)l.tiles, a.nseg - 1, D);
-    if (a.lengths) recurrence_segment_kernel<E, VEC, true, BACK><<<before, kW * 64, 0, s>>>(a);
-    else recurrence_segment_kernel<E, VEC, false, BACK><<<before, kW * 64, 0, s>>>(a);
+  // More tiles than a grid takes (2^32 threads) go in launches of nearly equal parts; time is not cut then.
+  const long most = (1L << 32) / (kW * 64) - 1, parts = (l.tiles + most - 1) / most, per = (l.tiles + parts - 1) / parts;
+  for (long tile = 0; tile < l.tiles; tile += per) {
+    a.tile0 = (unsigned)tile;
+    const unsigned tiles = (unsigned)std::min(per, l.tiles - tile);
+    const dim3 grid(tiles, a.nseg, D);
+    if (a.nseg > 1) {
+      const dim3 before(tiles, a.nseg - 1, D);
+      if (a.lengths) recurrence_segment_kernel<E, VEC, true, BACK><<<before, kW * 64, 0, s>>>(a);
+      else recurrence_segment_kernel<E, VEC, false, BACK><<<before, kW * 64, 0, s>>>(a);
+      AVC_LAUNCH_CHECK();
+    }
+    if constexpr (BACK) {
+      if (a.lengths) recurrence_backward_kernel<E, VEC, true><<<grid, kW * 64, 0, s>>>(a);
+      else recurrence_backward_kernel<E, VEC, false><<<grid, kW * 64, 0, s>>>(a);
+    } else {
+      if (a.lengths) recurrence_forward_kernel<E, VEC, true><<<grid, kW * 64, 0, s>>>(a);
+      else recurrence_forward_kernel<E, VEC, false><<<grid, kW * 64, 0, s>>>(a);
+    }
     AVC_LAUNCH_CHECK();
   }
-  if constexpr (BACK) {
-    if (a.lengths) recurrence_backward_kernel<E, VEC, true><<<grid, kW * 64, 0, s>>>(a);
-    else recurrence_backward_kernel<E, VEC, false><<<grid, kW * 64, 0, s>>>(a);
-  } else {
-    if (a.lengths) recurrence_forward_kernel<E, VEC, true><<<grid, kW * 64, 0, s>>>(a);
-    else recurrence_forward_kernel<E, VEC, false><<<grid, kW * 64, 0, s>>>(a);
-  }
-  AVC_LAUNCH_CHECK();
   return AVC_OK;
 }
 

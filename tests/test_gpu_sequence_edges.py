@@ -65,3 +65,20 @@ def test_a_gradient_of_a_gradient_is_an_error(cuda_device):
     want, = torch.autograd.grad(ops.dropout(g, 0.5, _rng(dev)).sum(), g)
     (loss + d.square().sum()).backward()
     assert torch.equal(g.grad, want)
+
+
+@pytest.mark.parametrize("dtype,H", [(torch.float32, 65), (torch.bfloat16, 129)], ids=["f32", "bf16"])
+def test_recurrence_of_more_row_tiles_than_a_grid_takes(cuda_device, dtype, H):
+    """Rows go in several launches: every row has what it has in a call of its neighbours alone."""
+    B = 2 ** 22 + 1003  # two channel tiles a row
+    g = torch.empty(B, 3 * H, dtype=dtype, device=cuda_device)
+    g.normal_(generator=torch.Generator(device=cuda_device).manual_seed(3)).requires_grad_(True)
+    y, hT = ops.gated_recurrence(g, 1, B)
+    d, = torch.autograd.grad((y, hT), g, (y.detach(), hT.detach()))
+    for lo in (0, B // 2 - 500, B - 1000):
+        rows = slice(lo, lo + 1000)
+        part = g.detach()[rows].clone().requires_grad_(True)
+        y2, hT2 = ops.gated_recurrence(part, 1, 1000)
+        assert torch.equal(y[rows], y2) and torch.equal(hT[:, rows], hT2)
+        assert torch.equal(d[rows], torch.autograd.grad((y2, hT2), part, (y2.detach(), hT2.detach()))[0])
+    assert bool((hT.abs() <= 1).all())
