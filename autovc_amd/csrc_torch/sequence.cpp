@@ -19,6 +19,7 @@
 #include <torch/extension.h>
 
 #include <algorithm>
+#include <climits>
 
 #include "../../include/autovc_hip.h"
 
@@ -112,14 +113,15 @@ void check_seen(const char* what, const T&... inputs) {
               what, " cannot be traced: it is no operator of torch's dispatcher");
 }
 
-// A matrix whose rows the kernels can walk: t itself unless its rows are not dense or overlap.
+// A matrix whose rows the kernels can walk: t itself unless its rows are not dense, overlap or lie `most`
+// elements apart or more.
 struct Rows {
   Tensor t;
   long ld;
-  explicit Rows(const Tensor& m) : t(m), ld(m.size(1)) {
+  explicit Rows(const Tensor& m, long most = LONG_MAX) : t(m), ld(m.size(1)) {
     if (m.is_contiguous()) return;
     const bool dense = m.size(1) <= 1 || m.stride(1) == 1, apart = m.size(0) <= 1 || m.stride(0) >= m.size(1);
-    if (!dense || !apart) t = m.contiguous();
+    if (!dense || !apart || (m.size(0) > 1 && m.stride(0) >= most)) t = m.contiguous();
     else if (m.size(0) > 1) ld = m.stride(0);
   }
   void* p() const { return t.data_ptr(); }
@@ -165,12 +167,14 @@ variable_list once(const variable_list& incoming, variable_list grads, bool line
 struct RecShape {
   long T, B, H, dirs;
   long D() const { return dirs == 3 ? 2 : 1; }
+  // row strides that the kernels' 32-bit offsets do not reach, where up to 64 rows share a wave
+  long too_far() const { return H >= 128 ? 1L << 29 : 1L << 23; }
 };
 
 std::tuple<Tensor, Tensor, Tensor> recurrence_forward(const Tensor& gates, const Tensor& h0, const Tensor& lengths,
                                                       const RecShape& s, bool keep) {
   const int dt = dtype_of(gates);
-  const Rows g(gates);
+  const Rows g(gates, s.too_far());
   const auto f32 = gates.options().dtype(at::kFloat);
   Tensor y = at::empty({s.T * s.B, s.D() * s.H}, gates.options()), hT = at::empty({s.D(), s.B, s.H}, f32), states;
   if (keep) states = at::empty({(long)lib.avc_gated_recurrence_states(s.T, s.B, s.H, s.dirs)}, f32);
@@ -201,7 +205,8 @@ struct GatedRecurrence : torch::autograd::Function<GatedRecurrence> {
     const RecShape s{v[0], v[1], v[2], v[3]};
     const at::NoGradGuard plain;
     const int dt = dtype_of(gates);
-    const Rows g(gates), dy(d[0].defined() ? d[0] : at::zeros({s.T * s.B, s.D() * s.H}, gates.options()));
+    const Rows g(gates, s.too_far());
+    const Rows dy(d[0].defined() ? d[0] : at::zeros({s.T * s.B, s.D() * s.H}, gates.options()), s.too_far());
     const Tensor dhT = d[1].defined() ? d[1].contiguous() : Tensor();
     Tensor dg = at::empty({s.T * s.B, s.D() * 3 * s.H}, gates.options()), dh0;
     if (v[4]) dh0 = at::empty({s.D(), s.B, s.H}, states.options());

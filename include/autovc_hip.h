@@ -422,8 +422,9 @@ int avc_wavernn_persist_eligible(int rows, int rnn_dims, int fc_dims);
  *            y and dgates are 0, and the state passes them unchanged
  *   y        [T*B] rows of stride ldy, a row holding [D][H]
  *   states   avc_gated_recurrence_states() floats, kept for the backward (NULL when there is none)
- * T >= 1.  The backward takes dy [T*B] rows and dhT [D][B][H] (NULL = 0) and writes dgates ([D][3][H]
- * per row, every row) and dh0 [D][B][H] (may be NULL).
+ * T >= 1; row strides are below 2^23 elements (2^29 where H >= 128).  The backward takes dy [T*B] rows
+ * and dhT [D][B][H] (NULL = 0) and writes dgates ([D][3][H] per row, every row) and dh0 [D][B][H] (may
+ * be NULL).
  * _step: one frame of every row, gates [B] rows [3][H], h -> h_out (h_out = h is allowed), y [B] rows. */
 size_t avc_gated_recurrence_states(int T, int B, int H, int dirs);
 size_t avc_gated_recurrence_workspace(int dtype, int T, int B, int H, int dirs);

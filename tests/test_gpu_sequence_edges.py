@@ -82,3 +82,18 @@ def test_recurrence_of_more_row_tiles_than_a_grid_takes(cuda_device, dtype, H):
         assert torch.equal(y[rows], y2) and torch.equal(hT[:, rows], hT2)
         assert torch.equal(d[rows], torch.autograd.grad((y2, hT2), part, (y2.detach(), hT2.detach()))[0])
     assert bool((hT.abs() <= 1).all())
+
+
+def test_recurrence_of_few_columns_in_a_very_wide_buffer(cuda_device):
+    """Row strides past what the kernels' 32-bit offsets reach."""
+    T, B, H = 3, 2, 1
+    wide = torch.full((T * B, (1 << 23) + 5), math.nan, device=cuda_device)
+    wide[:, 3:6] = torch.randn(T * B, 3, generator=torch.Generator().manual_seed(1)).to(cuda_device)
+    dense = wide[:, 3:6].clone()
+    got, want = [], []
+    for g, out in ((wide[:, 3:6], got), (dense, want)):
+        leaf = g.detach().requires_grad_(True)
+        y, hT = ops.gated_recurrence(leaf, T, B)
+        out += [y, hT, *torch.autograd.grad((y, hT), leaf, (y.detach(), hT.detach()))]
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)
