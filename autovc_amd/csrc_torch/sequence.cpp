@@ -113,12 +113,18 @@ void check_seen(const char* what, const T&... inputs) {
               what, " cannot be traced: it is no operator of torch's dispatcher");
 }
 
+// t with its values as they stand in memory (a view may be the negative of what it shows: the imaginary part
+// of a conjugate)
+Tensor as_stored(const Tensor& t) { return t.is_neg() ? t.resolve_neg() : t; }
+Tensor dense(const Tensor& t) { return as_stored(t).contiguous(); }
+
 // A matrix whose rows the kernels can walk: t itself unless its rows are not dense, overlap or lie `most`
 // elements apart or more.
 struct Rows {
   Tensor t;
   long ld;
-  explicit Rows(const Tensor& m, long most = LONG_MAX) : t(m), ld(m.size(1)) {
+  explicit Rows(const Tensor& given, long most = LONG_MAX) : t(as_stored(given)), ld(t.size(1)) {
+    const Tensor m = t;
     if (m.is_contiguous()) return;
     const bool dense = m.size(1) <= 1 || m.stride(1) == 1, apart = m.size(0) <= 1 || m.stride(0) >= m.size(1);
     if (!dense || !apart || (m.size(0) > 1 && m.stride(0) >= most)) t = m.contiguous();
@@ -207,7 +213,7 @@ struct GatedRecurrence : torch::autograd::Function<GatedRecurrence> {
     const int dt = dtype_of(gates);
     const Rows g(gates, s.too_far());
     const Rows dy(d[0].defined() ? d[0] : at::zeros({s.T * s.B, s.D() * s.H}, gates.options()), s.too_far());
-    const Tensor dhT = d[1].defined() ? d[1].contiguous() : Tensor();
+    const Tensor dhT = d[1].defined() ? dense(d[1]) : Tensor();
     Tensor dg = at::empty({s.T * s.B, s.D() * 3 * s.H}, gates.options()), dh0;
     if (v[4]) dh0 = at::empty({s.D(), s.B, s.H}, states.options());
     const size_t bytes = lib.avc_gated_recurrence_workspace(dt, s.T, s.B, s.H, s.dirs);
@@ -238,7 +244,7 @@ std::tuple<Tensor, Tensor> gated_recurrence(const Tensor& gates, long T, long B,
     check_type(*h0, "h0", gates, at::kFloat, at::kFloat);
     TORCH_CHECK_VALUE(h0->dim() == 3 && h0->size(0) == D && h0->size(1) == B && h0->size(2) == H, "h0 must be [", D, ", ", B,
                       ", ", H, "], got ", h0->sizes());
-    h0 = h0->contiguous();
+    h0 = dense(*h0);
   }
   Tensor len;
   if (lengths) {
@@ -283,7 +289,7 @@ std::tuple<Tensor, Tensor> gated_recurrence_step(const Tensor& gates, const Tens
     out = *out_state;
     check_type(out, "out_state", gates, at::kFloat, at::kFloat);
     TORCH_CHECK(!wants_grad(out), "out_state is written in place, so it cannot require a gradient");
-    TORCH_CHECK_VALUE(fits(out) && out.is_contiguous(), "out_state must be a contiguous [", B, ", ", H, "]");
+    TORCH_CHECK_VALUE(fits(out) && out.is_contiguous() && !out.is_neg(), "out_state must be a contiguous [", B, ", ", H, "]");
     TORCH_CHECK_VALUE(!overlap(out, state) || (out.data_ptr() == state.data_ptr() && state.is_contiguous()),
                       "out_state overlaps state without being it");
     TORCH_CHECK_VALUE(!overlap(out, gates), "out_state overlaps gates");
@@ -294,7 +300,7 @@ std::tuple<Tensor, Tensor> gated_recurrence_step(const Tensor& gates, const Tens
   Tensor y = at::empty({B, H}, gates.options());
   if (B) {
     const Rows g(gates);
-    const Tensor h = state.contiguous();
+    const Tensor h = dense(state);
     const On on(gates);
     done(lib.avc_gated_recurrence_step(dtype_of(gates), B, H, g.p(), g.ld, ptr<float>(h), ptr<float>(out), y.data_ptr(), H,
                                        on.stream),
@@ -346,7 +352,7 @@ struct TokenLogProbs : torch::autograd::Function<TokenLogProbs> {
     const long N = logits.size(0), V = logits.size(1);
     const Rows z(logits);
     Tensor dz = at::empty({N, V}, logits.options());
-    const Tensor dl = d[0].defined() ? d[0].contiguous() : Tensor(), de = d[1].defined() ? d[1].contiguous() : Tensor();
+    const Tensor dl = d[0].defined() ? dense(d[0]) : Tensor(), de = d[1].defined() ? dense(d[1]) : Tensor();
     if (N) {
       const On on(logits);
       done(lib.avc_token_log_probs_backward(dtype_of(logits), N, V, z.p(), z.ld, ptr<long long>(tokens),
@@ -393,7 +399,8 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> token_log_probs(Tensor logits, Tensor
 }
 
 // ---- counter-based dropout ----------------------------------------------------------------------------
-Tensor drop(const Tensor& x, const Tensor& residual, double p, const Tensor& rng, long layer) {
+Tensor drop(const Tensor& given, const Tensor& added, double p, const Tensor& rng, long layer) {
+  const Tensor x = as_stored(given), residual = added.defined() ? as_stored(added) : added;
   Tensor y = at::empty(x.sizes(), x.options());
   if (!x.numel()) return y;
   long n = 1, c = x.numel(), ldx = c, ldr = c;

@@ -97,3 +97,44 @@ def test_recurrence_of_few_columns_in_a_very_wide_buffer(cuda_device):
         out += [y, hT, *torch.autograd.grad((y, hT), leaf, (y.detach(), hT.detach()))]
     for a, b in zip(got, want):
         assert torch.equal(a, b)
+
+
+def test_negated_views(cuda_device):
+    """The imaginary part of a conjugate is a view whose memory holds the opposite sign."""
+    dev = cuda_device
+
+    def pair(*shape):
+        z = torch.randn(*shape, dtype=torch.complex64, generator=torch.Generator().manual_seed(len(shape))).to(dev)
+        v = z.conj().imag
+        assert v.is_neg()
+        return v, v.resolve_neg().contiguous()
+
+    tok = torch.zeros(1, dtype=torch.int64, device=dev)
+    v, p = pair(4, 1)
+    assert torch.equal(ops.dropout(v, 0.0, _rng(dev)), p)
+    assert torch.equal(ops.dropout(p, 0.0, _rng(dev), residual=v), p + p)
+    lone = torch._neg_view(p)
+    assert torch.equal(ops.dropout(lone, 0.0, _rng(dev)), -p)
+    v, p = pair(6, 9)
+    v, p = torch._neg_view(p), -p
+    leaf, dense = v.detach().requires_grad_(True), p.detach().requires_grad_(True)
+    s = torch._neg_view(torch.rand(1, 2, 3, device=dev))
+    y, hT = ops.gated_recurrence(leaf, 3, 2, h0=s)
+    y2, hT2 = ops.gated_recurrence(dense, 3, 2, h0=s.resolve_neg())
+    assert torch.equal(y, y2) and torch.equal(hT, hT2)
+    dy, dh = torch._neg_view(y2.detach()), torch._neg_view(hT2.detach())
+    d, = torch.autograd.grad((y, hT), leaf, (dy, dh))
+    d2, = torch.autograd.grad((y2, hT2), dense, (dy.resolve_neg(), dh.resolve_neg()))
+    assert torch.equal(d, d2)
+    a, b = ops.gated_recurrence_step(v[:2].detach(), s[0]), ops.gated_recurrence_step(p[:2], s[0].resolve_neg())
+    assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+    with pytest.raises(ValueError, match="out_state"):
+        ops.gated_recurrence_step(p[:2], torch.zeros(2, 3, device=dev), out_state=torch._neg_view(torch.zeros(2, 3, device=dev)))
+    tok = torch.arange(6, device=dev)
+    a, b = ops.token_log_probs(leaf, tok, top=2), ops.token_log_probs(dense, tok, top=2)
+    for k in range(4):
+        assert torch.equal(a[k], b[k])
+    gl, ge = torch._neg_view(torch.rand(6, device=dev)), torch._neg_view(torch.rand(6, device=dev))
+    d, = torch.autograd.grad(a[:2], leaf, (gl, ge))
+    d2, = torch.autograd.grad(b[:2], dense, (gl.resolve_neg(), ge.resolve_neg()))
+    assert torch.equal(d, d2)
