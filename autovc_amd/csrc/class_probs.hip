@@ -193,7 +193,9 @@ __device__ __forceinline__ void append(u64* list, int* count, int cap, bool in, 
 
 template <int GT>
 struct TopShared {
-  static constexpr int kCap = GT == 64 ? 128 : 256;  // candidates that are ranked at once
+  // Candidates that are ranked at once: all of a dense row with fewer than kMaxTop slices in a wave, 31 of 8
+  // classes at most (1x200 fp16 classes with 32 alternatives 17 us; with a list of 128, a class a round, 31)
+  static constexpr int kCap = 256;
   u64 cand[kCap];
   unsigned tau;
   int count, nsel;
@@ -254,7 +256,8 @@ __device__ void select_top(TopShared<GT>& sh, int tid, int k, unsigned mine, con
       }
     }
   };
-  // (tau stands at -inf where fewer than k classes are left: all the others are equal then)
+  // (tau is -inf's where fewer than k classes are left, all the others being equal then, and below it, at 1,
+  // where no wave has k slices: every class is above it)
   if (tau > value_bits(-INFINITY)) {
     slices([&](bool in, float x, long c) {
       append(sh.cand, &sh.count, kCap, in && value_bits(x) >= tau, class_key(x, c));

@@ -29,6 +29,18 @@ def test_log_probs_of_classes_a_subnormal_apart(cuda_device, dtype, N, V):
 
 
 @pytest.mark.parametrize("dtype", TYPES, ids=IDS)
+@pytest.mark.parametrize("N,V", [(1, 130), (2, 200), (3, 248), (2, 124), (3, 3 * 4096 + 200), (2, 2 ** 16 + 216)])
+def test_log_probs_with_fewer_slices_than_alternatives(cuda_device, dtype, N, V):
+    """Rows, and last segments of rows, of fewer vectors than alternatives, with and without equal classes."""
+    gen = torch.Generator().manual_seed(V)
+    tok = torch.randint(0, V, (N,), generator=gen)
+    for z in (torch.randn(N, V, generator=gen), torch.randint(0, 3, (N, V), generator=gen).float(),
+              torch.linspace(-2, 2, V).expand(N, V), torch.randn(N, V, generator=gen).masked_fill(torch.arange(V) % 3 > 0, -math.inf)):
+        for top in (17, 31, 32):
+            _check_log_probs(cuda_device, z.to(dtype), tok, top)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS)
 def test_recurrence_state_of_small_candidates(cuda_device, dtype):
     """The fp32 state of one frame is as exact for 16-bit gates as for fp32 ones: with the forget gate at 1/2
     the state is tanh(c) / 2, off by at most 16 units: the candidate's 12 (a reciprocal, a sum and an
