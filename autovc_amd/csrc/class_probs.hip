@@ -466,8 +466,7 @@ __global__ __launch_bounds__(GT * kRows<GT>) void class_probs_forward_kernel(Pro
 // which spares three quarters of what a row costs beside its classes (reductions, logarithms) -- with
 // a wave a row that is what bounds it.  35200 rows of 512 fp32 classes 14.6 us (4.9 TB/s, the rate of a
 // large copy), with a wave a row 19.9; with 5 alternatives 26 and 38; 60000 rows of 100 fp32 classes with
-// 5 alternatives 18 and 57.  (Many alternatives of 512
-// fp32 classes are the exception: 35200 rows with 32 47 and 45, 4096 with 20 11 and 9.)
+// 5 alternatives 18 and 57.  (Where it does not: short_rows.)
 constexpr int kShort = 512;
 constexpr int kShortCand = 64;  // candidates of a row that are ranked at once
 
@@ -746,9 +745,19 @@ __global__ __launch_bounds__(256) void class_probs_backward_kernel(ProbArgs a, c
   }
 }
 
-
-// (fewer rows than 4096 take 5 to 7 us either way)
-bool short_rows(long N, long V) { return V <= kShort && N >= 4096; }
+// Whether 16 lanes take a row (fewer rows than 4096 take 5 to 7 us either way).  With more than 16 alternatives
+// of more than kShort / 2 classes their list costs most, and a wave a row, which in fp32 has as many slices as
+// it can, is faster while rows are few or their classes many.  16 lanes and a wave, us, with 20 and 32:
+//   fp32  4096x300  10.1  8.9  11.6  9.6    8192x384  14.2 13.7  15.7 14.5    12000x384 18.0 18.0  19.4 19.3
+//         4096x512  11.1  9.1  12.5  9.6   12000x512  18.7 17.4  20.6 18.2    35200x512 41.4 40.1  45.8 42.5
+//        35200x300  37.7 40.8  41.8 42.9   35200x448  39.7 41.8  43.8 44.2
+//   bf16  4096x300  10.8 10.9  12.3 13.6    4096x512  11.0 10.2  12.4 10.8     8192x512 14.1 16.3  15.9 17.0
+// (4096x512 fp32 with 16: 9.6 and 8.8; 4096x256 with 32: 9.6 and 8.9.)
+bool short_rows(long N, long V, int top, int vec) {
+  if (V > kShort) return false;
+  if (top <= 16 || V <= kShort / 2) return N >= 4096;
+  return vec == 4 ? N >= 12000 && V <= 448 : N >= (V <= 384 ? 4096 : 8192);
+}
 
 // A wave takes a row where rows are short, or many enough to fill the chip so (4096 rows of 50001
 // bf16 classes: 83 us, with a workgroup a row 90); else a workgroup does.
@@ -803,7 +812,7 @@ int in_parts(const ProbArgs& all, long most, Launch launch) {
 
 template <typename E, bool TOP>
 int run_forward(ProbArgs a, hipStream_t s) {
-  if (short_rows(a.N, a.V)) {
+  if (short_rows(a.N, a.V, a.top, width<E>())) {
     constexpr int most = kShort / 16 / width<E>();  // vectors a lane
     const unsigned grid = (unsigned)((a.N + 15) / 16);
     if (a.V <= kShort / 4) class_probs_short_kernel<E, most / 4, TOP><<<grid, 256, 0, s>>>(a);

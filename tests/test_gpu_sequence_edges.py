@@ -40,6 +40,25 @@ def test_log_probs_with_fewer_slices_than_alternatives(cuda_device, dtype, N, V)
             _check_log_probs(cuda_device, z.to(dtype), tok, top)
 
 
+@pytest.mark.parametrize("dtype,N,V", [(torch.float32, 12007, 440), (torch.float32, 12000, 300), (torch.bfloat16, 8200, 500),
+                                       (torch.float16, 8192, 512), (torch.float16, 4100, 384)])
+@pytest.mark.parametrize("top", [17, 32])
+def test_log_probs_many_short_rows_with_many_alternatives(cuda_device, dtype, N, V, top):
+    """Neighbouring rows of different kinds where 16 lanes hold a row and rank from their four largest each."""
+    gen = torch.Generator().manual_seed(V + top)
+    z = torch.randn(N, V, generator=gen)
+    z[1::9] = 0.25
+    z[2::9] = torch.randint(0, 3, (len(z[2::9]), V), generator=gen).float()
+    z[3::9, 5:] = -math.inf
+    z[4::9] = -math.inf
+    z[5::9] = torch.linspace(-4, 4, V)
+    lane = torch.arange(V) // (4 if dtype == torch.float32 else 8) % 16
+    z[6::9] = torch.where((lane >= 1) & (lane <= 3), z[6::9], torch.tensor(-math.inf))
+    z[7::9] = torch.where(lane == 9, z[7::9].round(), z[7::9] - 20.0)
+    z[8::9, 100] = 25.0
+    _check_log_probs(cuda_device, z.to(dtype), torch.randint(0, V, (N,), generator=gen), top)
+
+
 @pytest.mark.parametrize("dtype", TYPES, ids=IDS)
 def test_recurrence_state_of_small_candidates(cuda_device, dtype):
     """The fp32 state of one frame is as exact for 16-bit gates as for fp32 ones: with the forget gate at 1/2
