@@ -11,13 +11,14 @@ SRC      := $(wildcard autovc_amd/csrc/*.hip)
 HDR      := $(wildcard autovc_amd/csrc/*.h) include/autovc_hip.h include/autovc_hip_debug.h
 OBJ      := $(patsubst autovc_amd/csrc/%.hip,build/%.o,$(SRC))
 LIB      := autovc_amd/libautovc_hip.so
-# the sequence-model operators as torch functions (a Python module over the C ABI, no GPU code)
+# the sequence-model operators as torch functions (a Python module over the C ABI, no GPU code);
+# built where $(PY) has torch
 EXT      := autovc_amd/_sequence.so
 PY       ?= python3
-TORCH    := $(shell $(PY) -c "import importlib.util as u, os; print(os.path.dirname(u.find_spec('torch').origin))")
+TORCH    := $(shell $(PY) -c "import importlib.util as u, os; s = u.find_spec('torch'); print(os.path.dirname(s.origin) if s else '')")
 PYINC    := $(shell $(PY) -c "import sysconfig; print(sysconfig.get_paths()['include'])")
 
-all: $(LIB) $(EXT)
+all: $(LIB) $(if $(TORCH),$(EXT))
 
 $(EXT): autovc_amd/csrc_torch/sequence.cpp include/autovc_hip.h Makefile
 	$(CXX) -O2 -std=c++17 -fPIC -shared -Wall -Wno-sign-compare -D__HIP_PLATFORM_AMD__=1 -DUSE_ROCM=1 \
