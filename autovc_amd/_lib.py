@@ -211,13 +211,7 @@ def context(device: torch.device) -> int:
     return ctx
 
 
-# the current stream's handle without a Stream object around it (2 us less a call)
-_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
-
-
 def stream(device: torch.device) -> int:
-    if _raw_stream is not None and device.index is not None:
-        return _raw_stream(device.index)
     return torch.cuda.current_stream(device).cuda_stream
 
 
