@@ -23,7 +23,7 @@ def recurrence(gates, T, B, h0=None, lengths=None, dirs=1):
     """y [T*B][D*H] and hT [D][B][H] by the definition, frame by frame (differentiable)."""
     D = 2 if dirs == 3 else 1
     H = gates.shape[1] // (3 * D)
-    g = gates.double().view(T, B, D, 3, H)
+    g = gates.double().view(T, B, D, 3, H).unbind(0)  # (a frame taken by its index would cost its gradient T frames)
     length = [T] * B if lengths is None else [max(0, min(T, int(v))) for v in lengths]
     live = torch.tensor([[t < length[b] for b in range(B)] for t in range(T)]).view(T, B, 1)
     ys, hs = [], []
@@ -32,7 +32,7 @@ def recurrence(gates, T, B, h0=None, lengths=None, dirs=1):
         h = torch.zeros(B, H, dtype=torch.float64) if h0 is None else h0[d].double()
         y = [None] * T
         for t in (range(T - 1, -1, -1) if rev else range(T)):
-            pre = torch.where(live[t][:, None], g[t, :, d], torch.zeros((), dtype=torch.float64))
+            pre = torch.where(live[t][:, None], g[t][:, d], torch.zeros((), dtype=torch.float64))
             f, z, o = torch.sigmoid(pre[:, 0]), torch.tanh(pre[:, 1]), torch.sigmoid(pre[:, 2])
             h = torch.where(live[t], f * h + torch.sigmoid(-pre[:, 0]) * z, h)
             y[t] = torch.where(live[t], o * h, torch.zeros((), dtype=torch.float64))

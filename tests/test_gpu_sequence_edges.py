@@ -4,9 +4,9 @@ import math
 import pytest
 import torch
 
-from autovc_amd import ops
+from autovc_amd import _lib, ops
 from oracle import sequence_oracle as so
-from tests.test_gpu_sequence import IDS, TYPES, _check_log_probs, _near, _rng
+from tests.test_gpu_sequence import IDS, TYPES, _check_log_probs, _check_recurrence, _near, _rng
 
 pytestmark = pytest.mark.gpu
 
@@ -169,3 +169,29 @@ def test_negated_views(cuda_device):
     d, = torch.autograd.grad(a[:2], leaf, (gl, ge))
     d2, = torch.autograd.grad(b[:2], dense, (gl.resolve_neg(), ge.resolve_neg()))
     assert torch.equal(d, d2)
+
+
+def _segments(dtype, T, B, H, dirs):
+    """Segments that time is cut into, of the pass that cuts it finer."""
+    D = 2 if dirs == 3 else 1
+    return _lib.load().avc_gated_recurrence_workspace(_lib.DTYPES[dtype], T, B, H, dirs) // (2 * D * B * H * 4)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS)
+@pytest.mark.parametrize("T,B,H,dirs,ragged", [
+    (1100, 60, 66, 1, False), (1100, 60, 66, 3, True), (1030, 64, 130, 2, True), (1024, 64, 130, 1, False), (2050, 20, 34, 3, True)])
+def test_recurrence_segments_of_several_chunks(cuda_device, dtype, T, B, H, dirs, ragged):
+    """Segments of 2 to 9 chunks, so that a wave's run of a segment is longer than its frames in flight, with
+    and without a rest, and a workgroup goes on over several chunks behind the joined segments."""
+    n = _segments(dtype, T, B, H, dirs)
+    chunk = 64 if dtype == torch.float32 else 32  # the finer pass's
+    assert n > 1 and -(-T // chunk) >= 2 * n
+    lengths = [(T, 0, T - 1, T // 2 + 3, 1, 700, 63)[b % 7] for b in range(B)] if ragged else None
+    _check_recurrence(cuda_device, dtype, T, B, H, dirs, lengths, h0=True)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS)
+@pytest.mark.parametrize("T,B,H,dirs,pad", [(20, 40, 130, 1, 0), (9, 31, 200, 3, 7), (70, 16, 128, 2, 5), (600, 11, 130, 3, 7)])
+def test_recurrence_of_many_channel_tiles(cuda_device, dtype, T, B, H, dirs, pad):
+    """Rows of several channel tiles that begin inside a cache line, in a grid that is reordered in part."""
+    _check_recurrence(cuda_device, dtype, T, B, H, dirs, [T - b % 5 for b in range(B)], True, pad)
