@@ -98,12 +98,16 @@ class GatedRecurrence(nn.Module):
 
     def forward(self, x, T, B, h0=None, lengths=None):
         """x [T*B][input_size] -> (y [T*B][D*H], last states [D][B][H]); see ops.gated_recurrence."""
-        return ops.gated_recurrence(ops.Linear.apply(x, self.weight_ih, self.bias_ih), T, B, h0, lengths, self.dirs)
+        return ops.gated_recurrence(self._gates(x), T, B, h0, lengths, self.dirs)
 
     @torch.no_grad()
     def step(self, x, state):
         """One frame of a forward layer, state [B][H] updated in place: x [B][input_size] -> y [B][H]."""
         if self.dirs != 1:
             raise ValueError("only a forward layer can be stepped")
-        gates = ops.Linear.apply(x, self.weight_ih, self.bias_ih)
-        return ops.gated_recurrence_step(gates, state, out_state=state)[0]
+        return ops.gated_recurrence_step(self._gates(x), state, out_state=state)[0]
+
+    def _gates(self, x):
+        if x.shape[0] == 0:  # no frame: nothing to launch, and no gradient but zero
+            return nn.functional.linear(x, self.weight_ih, self.bias_ih)
+        return ops.Linear.apply(x, self.weight_ih, self.bias_ih)

@@ -87,3 +87,15 @@ def test_wavernn_log_probs(cuda_device):
     assert math.isfinite(top_logp.sum().item())
     with pytest.raises(ValueError):
         WaveRNN(device=cuda_device, mode="MOL").log_probs(x, mels, classes)
+
+
+@pytest.mark.parametrize("T,B", [(0, 3), (5, 0)])
+def test_gated_recurrence_layer_without_frames(cuda_device, T, B):
+    layer = GatedRecurrence(8, 12, bidirectional=True).to(cuda_device)
+    h0 = torch.rand(2, B, 12, device=cuda_device)
+    y, hT = layer(torch.zeros(0, 8, device=cuda_device, requires_grad=True), T, B, h0=h0)
+    assert y.shape == (0, 24) and torch.equal(hT, h0)
+    (y.sum() + hT.sum()).backward()
+    assert all((p.grad == 0).all() for p in layer.parameters())
+    y = GatedRecurrence(8, 12).to(cuda_device).step(torch.zeros(0, 8, device=cuda_device), torch.zeros(0, 12, device=cuda_device))
+    assert y.shape == (0, 12)
