@@ -367,7 +367,8 @@ __device__ __forceinline__ void emit_top(const ProbArgs& a, long row, int r, u64
 
 // GT threads a row segment: a wave, four of them a workgroup, or a workgroup of 256 (blockIdx.y is
 // the segment).  A thread reads U vectors at a time and asks for the next U before it adds the first.
-// Bound by the one read of the logits: 4096 rows of 50001 bf16 classes 83 us, 4.9 TB/s.  Few rows are
+// Bound by the one read of the logits: 4096 rows of 50001 bf16 classes alone 83 us, 4.9 TB/s (73 traced);
+// in a training pass, behind a backward whose writes are still on their way to memory, 106.  Few rows are
 // bound by the chain of load, reduction and store: one of 512 fp32 classes with 5 alternatives 5 us.
 template <int GT>
 constexpr int kRows = GT == 64 ? 4 : 1;  // rows of a workgroup
@@ -647,7 +648,7 @@ __global__ __launch_bounds__(256) void class_probs_short_kernel(ProbArgs a) {
 
 // One workgroup a row: the first wave joins the segments' statistics (a lane a segment); of the
 // segments' lists the keys that can be among the first `top` are ranked.  5 rows of 151001 fp16 classes
-// with 20 alternatives: 9 us for the segments and 5 for this, both chains of a few dependent steps.
+// with 20 alternatives: 9 to 10 us for the segments and 5.6 for this, both chains of a few dependent steps.
 template <typename E>
 __global__ __launch_bounds__(256) void class_probs_join_kernel(ProbArgs a) {
   const long row = blockIdx.x;
@@ -760,7 +761,7 @@ bool short_rows(long N, long V, int top, int vec) {
 }
 
 // A wave takes a row where rows are short, or many enough to fill the chip so (4096 rows of 50001
-// bf16 classes: 83 us, with a workgroup a row 90); else a workgroup does.
+// bf16 classes alone: 83 us, with a workgroup a row 90); else a workgroup does.
 bool wave_rows(long N, long V) { return V <= 2048 || N >= 4096; }
 
 // Segments of a row: where there are few long rows (below 16 rounds of a workgroup the second launch

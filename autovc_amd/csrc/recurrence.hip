@@ -195,7 +195,8 @@ __device__ void join_segments(const RecArgs& a, int lo, int hi, const float* agg
 // A workgroup walks its segment chunk by chunk: each wave forms its stretch's action from gates that were
 // asked for a chunk earlier, the actions meet in LDS (double-buffered: one barrier a chunk), and each
 // wave goes over its own stretch, still in registers, with the state that comes to it.  Gates are read
-// once and y written once: 128x256x512 fp32 55 us (4.9 TB/s, the rate of a large copy), bf16 31 us.
+// once and y written once: 128x256x512 alone fp32 55 us (4.9 TB/s, the rate of a large copy), bf16 32; in a
+// training pass, behind a backward whose writes are still on their way to memory, fp32 69.
 template <typename E, int VEC, bool RAGGED>
 __global__ __launch_bounds__(kW * 64, 4) void recurrence_forward_kernel(RecArgs a) {
   constexpr int kS = stretch<VEC, false>(), kChunk = kS * kW;
@@ -288,8 +289,8 @@ __global__ __launch_bounds__(kW * 64, 4) void recurrence_forward_kernel(RecArgs 
 
 // The same walk from the last chunk to the first, with the action on the state too (from the state kept
 // at the chunk's beginning), so that h needs no pass of its own.  Bound by reading gates and dy and
-// writing dgates once: 128x256x512 fp32 102 us (4.6 TB/s; 87 right behind the forward, which leaves some
-// of the gates in the last-level cache), bf16 48 us.
+// writing dgates once: 128x256x512 alone fp32 102 us (4.6 TB/s; 88 right behind the forward, which leaves
+// some of the gates in the last-level cache), bf16 49 us.
 template <typename E, int VEC, bool RAGGED>
 __global__ __launch_bounds__(kW * 64, 2) void recurrence_backward_kernel(RecArgs a) {
   constexpr int kS = stretch<VEC, true>(), kChunk = kS * kW;
@@ -433,11 +434,11 @@ __global__ __launch_bounds__(kW * 64, 2) void recurrence_backward_kernel(RecArgs
 
 // What one segment of time does to the state before it (BACK: to the gradient behind it): each
 // wave walks a run of stretches of its own, then the waves' runs are joined in order.  It reads two
-// thirds of the gates (60001x1x500 fp16: 36 us, then 60 us for the forward).  One pass in which the
+// thirds of the gates (60001x1x500 fp16: 40 us, then 60 us for the forward).  One pass in which the
 // workgroups hand the state on as they go read them once and took longer: 137 us instead of 111 then.
 template <typename E, int VEC, bool RAGGED, bool BACK>
 __global__ __launch_bounds__(kW * 64, 6) void recurrence_segment_kernel(RecArgs a) {
-  constexpr int kS = 16;  // frames in flight (with 4 the ragged backward's took 17 us, with 16 it takes 15)
+  constexpr int kS = 16;  // frames in flight (1024x32x256, both directions, ragged, bf16: 46 + 62 us, with 4 47.5 + 64)
   const Place<E, VEC> at(a);
   const int wave = at.wave, lane = at.lane;
   __shared__ float part[kW][2][64][VEC];
@@ -513,7 +514,7 @@ __global__ __launch_bounds__(kW * 64, 6) void recurrence_segment_kernel(RecArgs 
   }
 }
 
-// One frame of every row: the served form.  Bound by its launch (512 channels 1.9 us).
+// One frame of every row: the served form.  Bound by its launch (512 channels 2.0 us).
 template <typename E, int VEC>
 __global__ __launch_bounds__(256) void recurrence_step_kernel(int B, int H, const E* gates, long ldg, const float* h,
                                                               float* h_out, E* y, long ldy) {
@@ -561,8 +562,8 @@ __global__ __launch_bounds__(256) void recurrence_step_kernel(int B, int H, cons
 }
 
 // Channels of a lane: 4 bytes.  (8-byte lanes hold twice the registers: a training pass of
-// 128x256x512 takes 89 + 98 us in fp32 instead of 55 + 102, 76 + 55 us in bf16 instead of 31 + 48;
-// 2-byte lanes of 16-bit gates 37 + 55.)
+// 128x256x512 takes 88 + 98 us in fp32 instead of 55 + 102, 77 + 56 us in bf16 instead of 32 + 49;
+// 2-byte lanes of 16-bit gates 37 + 56.)
 template <typename E>
 constexpr int wide() { return sizeof(E) == 4 ? 1 : 2; }
 
@@ -570,9 +571,9 @@ constexpr int wide() { return sizeof(E) == 4 ? 1 : 2; }
 // enough to fill the chip each workgroup walks its rows' whole time; with fewer, time is cut into as
 // many segments as bring the grid to two workgroups a CU, which costs a pass over most of the gates
 // for the segments' actions and a launch.  1024 frames in 128 tiles (bf16, ragged): cut in four
-// 42 us, in two 49, whole 57; 60001 frames in 4 tiles: 128 segments 93 us, 64 106; twice as many segments
-// 43 and, in launch order, 107 (128: 100).  Up to 512 frames are not
-// cut: 400 frames in 180 tiles 36 us cut, 26 whole; 200 frames in 16 tiles 13 us either way.
+// 46 us, in two 53, whole 61; 60001 frames in 4 tiles: 128 segments 95 us, 64 107; twice as many segments
+// 48 and 100.  Up to 512 frames are not cut: 400 frames in 180 tiles 36 us cut, 26 whole; 200 frames in 16
+// tiles 13 us either way.
 struct Layout {
   int log_g = 0, nct, nseg, seg_chunks;
   long tiles;
@@ -605,7 +606,7 @@ int run_recurrence(RecArgs a, size_t ws_bytes, hipStream_t s) {
   const long widest = std::max(a.ldg, std::max(a.ldy, std::max(a.lddy, a.lddg)));
   AVC_CHECK_ARG(widest < (1L << 29) >> (6 - l.log_g), "row stride too large");
   // Tiles that begin inside a 128-byte line share it with their neighbours: they then run on one XCD,
-  // whose L2 reads it once (60001 frames of 500 fp16 channels: 93 + 145 us, in launch order 100 + 165;
+  // whose L2 reads it once (60001 frames of 500 fp16 channels: 95 + 146 us, in launch order 101 + 165;
   // with tiles on whole lines the reordering only costs, 1 us of 37 + 59).
   const long line = 128 / (long)sizeof(E);
   const bool split = a.H % line || a.ldg % line || reinterpret_cast<uintptr_t>(a.gates) % 128;
