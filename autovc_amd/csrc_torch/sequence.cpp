@@ -157,10 +157,9 @@ bool wants_grad(const Tensor& a, const optional<Tensor>& b) {
 variable_list once(const variable_list& incoming, variable_list grads, bool linear = false) {
   if (!at::GradMode::is_enabled()) return grads;
   torch::autograd::edge_list edges = torch::autograd::collect_next_edges(incoming);
-  if (!linear) {
-    const auto& inputs = torch::autograd::get_current_node()->next_edges();
-    edges.insert(edges.end(), inputs.begin(), inputs.end());
-  }
+  // (a compiled backward runs without a node)
+  if (const auto node = linear ? nullptr : torch::autograd::get_current_node())
+    edges.insert(edges.end(), node->next_edges().begin(), node->next_edges().end());
   if (std::none_of(edges.begin(), edges.end(), [](const auto& e) { return e.is_valid(); })) return grads;
   auto error = std::make_shared<torch::autograd::Error>(
       "trying to differentiate twice a function whose gradient is not differentiable", std::move(edges));

@@ -195,3 +195,20 @@ def test_recurrence_segments_of_several_chunks(cuda_device, dtype, T, B, H, dirs
 def test_recurrence_of_many_channel_tiles(cuda_device, dtype, T, B, H, dirs, pad):
     """Rows of several channel tiles that begin inside a cache line, in a grid that is reordered in part."""
     _check_recurrence(cuda_device, dtype, T, B, H, dirs, [T - b % 5 for b in range(B)], True, pad)
+
+
+def test_a_compiled_backward(cuda_device):
+    """Run by a compiled graph, where no autograd node is current."""
+    g = torch.randn(12, 9, device=cuda_device, requires_grad=True)
+    tok = torch.zeros(12, dtype=torch.int64, device=cuda_device)
+
+    def loss():
+        y, hT = ops.gated_recurrence(g, 6, 2)
+        logp, entropy, _, _ = ops.token_log_probs(ops.dropout(g, 0.5, _rng(cuda_device)), tok)
+        return y.sum() + hT.sum() + logp.sum() + entropy.sum()
+
+    want, = torch.autograd.grad(loss(), g)
+    value = loss()
+    with torch._dynamo.compiled_autograd._enable(torch.compile(backend="eager")):
+        value.backward()
+    assert torch.equal(g.grad, want)
